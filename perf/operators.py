@@ -190,8 +190,9 @@ def prepare(case, seed):
 # ------------------------------------------------------------------ plain forms
 
 def _row_scale(x):
-    """A row's scale in an 8-bit cache: its largest magnitude becomes 127."""
-    return (x.float().abs().amax(-1) / 127.0).clamp_min(2.0 ** -126)
+    """A row's scale in an 8-bit cache: its largest magnitude becomes 127.  (Divided
+    in 64 bits: in 32, torch multiplies by a reciprocal on the GPU.)"""
+    return (x.abs().amax(-1).double() / 127.0).float().clamp_min(2.0 ** -126)
 
 
 def _padded(st):
