@@ -16,7 +16,8 @@
  *     (NULL = the null stream) and return without synchronising.
  *   - Host entry points take host pointers in the reference's per-sequence
  *     layout and return after the results are in host memory.
- *   - All tensors are fp32, and so is the arithmetic: contractions run on fp32
+ *   - All tensors are fp32 (those of the packed and paged entry points have an
+ *     element type), and so is the arithmetic: contractions run on fp32
  *     MFMAs, or on bf16 MFMAs with each fp32 in three bf16 parts (exactly) and
  *     the six products that reach fp32 precision accumulated in fp32: what is
  *     left out is below one fp32 rounding of each product.
@@ -40,6 +41,12 @@ extern "C" {
 #define WHA_ERR_HIP (-3)         /* a HIP runtime call failed                */
 #define WHA_ERR_WORKSPACE (-4)   /* caller workspace too small               */
 #define WHA_ERR_NOMEM (-5)       /* device or host allocation failed         */
+
+/* Element types of the packed and paged entry points. */
+#define WHA_F32 0
+#define WHA_BF16 1
+#define WHA_F16 2
+#define WHA_I8 3 /* caches only: 8-bit rows with an fp32 scale each */
 
 /* Strided view of B*H independent [T][D] matrices: element (b,h,t,d) of a
  * tensor with base pointer p is p[b*stride_b + h*stride_h + t*stride_t + d]
@@ -422,6 +429,111 @@ size_t wha_wave_kv_decode_workspace_size(const wha_wave_shape* shape, int32_t ca
 int wha_wave_kv_decode(const float* x, const wha_wave_weights* w, const wha_wave_shape* shape,
                        const wha_wave_kv_cache* kv, const int32_t* lengths, float* out, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- packed sequences and paged caches
+ * Serving and training on many sequences at once: attention of packed prompts
+ * with grouped heads (forward and backward), and a key-value cache in pages with
+ * its writer, its reader and the attention of one new token over it.  No
+ * counterpart in the reference, whose attention takes one sequence of one head
+ * layout; the mathematics is attention_cpu's (src/common/compute.rs:377-409) and
+ * attention_backward_single's (src/cpu/backward.rs:313-363).
+ *
+ * Tensors here have an element type; sums, softmax statistics and lse are fp32
+ * in all of them, and a result is rounded once (the probabilities, and in the
+ * backward the score gradients, also once to the element type as MFMA operands). */
+/* Causal attention of n_seq sequences packed one after the other: rows
+ * cu_seqlens[i] .. cu_seqlens[i+1] - 1 of q, k, v and o are sequence i
+ * (cu_seqlens: device, n_seq + 1 entries, not decreasing, from 0 to at most the
+ * row count; sequences of length 0 allowed).  Rows behind the last sequence are
+ * neither read nor written.  Layouts describe [T rows][H heads][D] views: B = 1,
+ * T = the row count (the same in all four), one D up to 128; q_layout->H query
+ * heads, k_layout->H = v_layout->H key-value heads, which must divide them (at
+ * most 128 query heads to one); query head h uses key-value head h / (H / Hkv).
+ * The views may be columns of one fused projection's rows.  lse [H][T], natural
+ * log, may be NULL.  Row count x query heads must be below 2^31 - 2^16.
+ * An infinity or NaN in a row reaches that row's and later rows' outputs of its
+ * own sequence, never an earlier one's.  cu_seqlens entries outside [0, T] are
+ * taken as 0 or T; with entries that decrease the outputs are unspecified, but
+ * nothing outside the tensors is read or written. */
+int wha_packed_fwd(const void* q, const void* k, const void* v, void* o,
+                   float* lse, const int32_t* cu_seqlens, int32_t n_seq,
+                   int32_t dtype, const wha_layout* q_layout,
+                   const wha_layout* k_layout, const wha_layout* v_layout,
+                   const wha_layout* o_layout, float scale, void* stream);
+
+/* Bytes of device workspace wha_packed_bwd needs (two floats per row and query
+ * head; 0 for an invalid layout). */
+size_t wha_packed_bwd_workspace_size(const wha_layout* q_layout);
+
+/* Its backward from the forward's o and lse: dq, dk, dv (overwritten; dk and dv
+ * summed over the query heads of a group) in the layouts of q, k and v, d_o in
+ * that of o.  The gradients must not overlap each other or the inputs.
+ * WHA_F32 and WHA_BF16; WHA_F16 is WHA_ERR_UNSUPPORTED: score gradients of a few
+ * thousand keys lie below its smallest number.  Deterministic (no atomics).
+ * workspace as for wha_attn_bwd. */
+int wha_packed_bwd(const void* q, const void* k, const void* v, const void* o,
+                   const void* d_o, const float* lse, void* dq, void* dk,
+                   void* dv, const int32_t* cu_seqlens, int32_t n_seq,
+                   int32_t dtype, void* workspace, size_t workspace_bytes,
+                   const wha_layout* q_layout, const wha_layout* k_layout,
+                   const wha_layout* v_layout, const wha_layout* o_layout,
+                   float scale, void* stream);
+
+/* Paged cache: k_cache and v_cache [n_pages][n_kv_head][page_size][D] contiguous,
+ * of the element type or WHA_I8; page_size a power of two up to 4096.  With
+ * WHA_I8, k_scale and v_scale [n_pages][n_kv_head][page_size] fp32 (else NULL):
+ * a row x is held as c, x ~ c * scale, with scale = max(max|x| / 127, 2^-126) and
+ * c = x / scale to the nearest integer, ties to even; a row that holds an
+ * infinity or NaN gets the scale NaN (it reads back as NaN).
+ *
+ * Slot s is place s % page_size of page s / page_size, in every head. */
+
+/* Rows k and v [T][n_kv_head][D] (layouts with B = 1, H = n_kv_head) into the
+ * slots slots[0 .. T-1] (device).  Rows whose slot is negative (padding) or past
+ * the last page are left out.  The slots must differ: of rows that name the same
+ * slot the cache holds a mixture. */
+int wha_paged_kv_write(const void* k, const void* v, const int64_t* slots,
+                       void* k_cache, void* v_cache, float* k_scale,
+                       float* v_scale, int32_t dtype, int32_t cache_dtype,
+                       int64_t n_pages, int32_t page_size,
+                       const wha_layout* k_layout, const wha_layout* v_layout,
+                       void* stream);
+
+/* The rows of slots[0 .. T-1] out of the cache again, as the numbers they stand
+ * for; zeros for slots that are negative or past the last page.  A slot may be
+ * named any number of times. */
+int wha_paged_kv_read(const void* k_cache, const void* v_cache,
+                      const float* k_scale, const float* v_scale,
+                      const int64_t* slots, void* k, void* v, int32_t dtype,
+                      int32_t cache_dtype, int64_t n_pages, int32_t page_size,
+                      const wha_layout* k_layout, const wha_layout* v_layout,
+                      void* stream);
+
+/* Bytes of device workspace wha_paged_decode needs (0: none). */
+size_t wha_paged_decode_workspace_size(const wha_layout* q_layout,
+                                       int32_t n_kv_head, int32_t page_size,
+                                       int32_t max_pages);
+
+/* Attention of one query per sequence over its cached positions 0 ..
+ * lengths[b] - 1: position i lies at place i % page_size of page
+ * block_table[b * table_stride + i / page_size].  q, o: [B][H][D] (layouts with
+ * T = 1, B sequences, H query heads), lse [B][H] or NULL.  block_table (max_pages
+ * entries a row are read at most) and lengths are device arrays, so a captured
+ * call serves a growing cache.  A length of 0 or less: o = 0, lse = -infinity.
+ * A sequence whose table names a page outside [0, n_pages) below its length, or
+ * whose length exceeds max_pages * page_size, gets NaN; nothing outside the cache
+ * is read.  Entries of the table past a sequence's length, and places of the cache
+ * past it, may hold anything.  max_pages * page_size at most 2^30.  Deterministic.
+ * workspace as for wha_attn_bwd (split partials). */
+int wha_paged_decode(const void* q, const void* k_cache, const void* v_cache,
+                     const float* k_scale, const float* v_scale,
+                     const int32_t* block_table, int64_t table_stride,
+                     int32_t max_pages, const int32_t* lengths, void* o,
+                     float* lse, void* workspace, size_t workspace_bytes,
+                     int32_t dtype, int32_t cache_dtype, int64_t n_pages,
+                     int32_t page_size, int32_t n_kv_head,
+                     const wha_layout* q_layout, const wha_layout* o_layout,
+                     float scale, void* stream);
 
 /* ---------------------------------------------------------------- inputs
  * Seeded synthetic inputs (host): continues the xorshift64 stream in *state

@@ -88,6 +88,34 @@ extern "C" {
     pub fn wha_host_wave_attention_backward(x: *const f32, d_attn_out: *const f32, w: *const WhaWaveWeights,
                                             t: i32, n_embd: i32, n_head: i32, content_dim: i32,
                                             g: *const WhaWaveGrads) -> c_int;
+    // packed sequences with grouped heads, and paged key-value caches
+    pub fn wha_packed_fwd(q: *const c_void, k: *const c_void, v: *const c_void, o: *mut c_void, lse: *mut f32,
+                          cu_seqlens: *const i32, n_seq: i32, dtype: i32, q_layout: *const WhaLayout,
+                          k_layout: *const WhaLayout, v_layout: *const WhaLayout, o_layout: *const WhaLayout,
+                          scale: f32, stream: *mut c_void) -> c_int;
+    pub fn wha_packed_bwd_workspace_size(q_layout: *const WhaLayout) -> usize;
+    pub fn wha_packed_bwd(q: *const c_void, k: *const c_void, v: *const c_void, o: *const c_void,
+                          d_o: *const c_void, lse: *const f32, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void,
+                          cu_seqlens: *const i32, n_seq: i32, dtype: i32, workspace: *mut c_void,
+                          workspace_bytes: usize, q_layout: *const WhaLayout, k_layout: *const WhaLayout,
+                          v_layout: *const WhaLayout, o_layout: *const WhaLayout, scale: f32,
+                          stream: *mut c_void) -> c_int;
+    pub fn wha_paged_kv_write(k: *const c_void, v: *const c_void, slots: *const i64, k_cache: *mut c_void,
+                              v_cache: *mut c_void, k_scale: *mut f32, v_scale: *mut f32, dtype: i32,
+                              cache_dtype: i32, n_pages: i64, page_size: i32, k_layout: *const WhaLayout,
+                              v_layout: *const WhaLayout, stream: *mut c_void) -> c_int;
+    pub fn wha_paged_kv_read(k_cache: *const c_void, v_cache: *const c_void, k_scale: *const f32,
+                             v_scale: *const f32, slots: *const i64, k: *mut c_void, v: *mut c_void, dtype: i32,
+                             cache_dtype: i32, n_pages: i64, page_size: i32, k_layout: *const WhaLayout,
+                             v_layout: *const WhaLayout, stream: *mut c_void) -> c_int;
+    pub fn wha_paged_decode_workspace_size(q_layout: *const WhaLayout, n_kv_head: i32, page_size: i32,
+                                           max_pages: i32) -> usize;
+    pub fn wha_paged_decode(q: *const c_void, k_cache: *const c_void, v_cache: *const c_void, k_scale: *const f32,
+                            v_scale: *const f32, block_table: *const i32, table_stride: i64, max_pages: i32,
+                            lengths: *const i32, o: *mut c_void, lse: *mut f32, workspace: *mut c_void,
+                            workspace_bytes: usize, dtype: i32, cache_dtype: i32, n_pages: i64, page_size: i32,
+                            n_kv_head: i32, q_layout: *const WhaLayout, o_layout: *const WhaLayout, scale: f32,
+                            stream: *mut c_void) -> c_int;
     pub fn wha_synth_normal(state: *mut u64, out: *mut f32, n: usize, stddev: f64, nthreads: c_int) -> c_int;
     pub fn wha_timing_enable(on: c_int) -> c_int;
     pub fn wha_timing_reset() -> c_int;

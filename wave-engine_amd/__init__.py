@@ -47,6 +47,8 @@ EXPORTED_SYMBOLS = (
     "wha_wave_kv_decode", "wha_host_wave_attention_forward", "wha_host_wave_attention_backward",
     "wha_linear_fwd", "wha_linear_bwd_dx", "wha_linear_bwd_dw_workspace_size", "wha_linear_bwd_dw",
     "wha_host_attention_core_fwd", "wha_host_attention_backward", "wha_host_attention",
+    "wha_packed_fwd", "wha_packed_bwd_workspace_size", "wha_packed_bwd",
+    "wha_paged_kv_write", "wha_paged_kv_read", "wha_paged_decode_workspace_size", "wha_paged_decode",
     "wha_synth_normal",
     "wha_timing_enable", "wha_timing_reset", "wha_timing_read",
 )
@@ -172,6 +174,16 @@ def lib():
         L.wha_wave_kv_decode_workspace_size.argtypes = [wsp, i32]
         L.wha_wave_kv_decode_workspace_size.restype = sz
         L.wha_wave_kv_decode.argtypes = [vp, wwp, wsp, kvp, ctypes.POINTER(ctypes.c_int32), vp, vp, sz, vp]
+        L.wha_packed_fwd.argtypes = [vp] * 6 + [i32, i32, lp, lp, lp, lp, ctypes.c_float, vp]
+        L.wha_packed_bwd_workspace_size.argtypes = [lp]
+        L.wha_packed_bwd_workspace_size.restype = sz
+        L.wha_packed_bwd.argtypes = [vp] * 10 + [i32, i32, vp, sz, lp, lp, lp, lp, ctypes.c_float, vp]
+        L.wha_paged_kv_write.argtypes = [vp] * 7 + [i32, i32, i64, i32, lp, lp, vp]
+        L.wha_paged_kv_read.argtypes = [vp] * 7 + [i32, i32, i64, i32, lp, lp, vp]
+        L.wha_paged_decode_workspace_size.argtypes = [lp, i32, i32, i32]
+        L.wha_paged_decode_workspace_size.restype = sz
+        L.wha_paged_decode.argtypes = [vp] * 6 + [i64, i32, vp, vp, vp, vp, sz, i32, i32, i64, i32, i32, lp, lp,
+                                                  ctypes.c_float, vp]
         L.wha_synth_normal.argtypes = [ctypes.POINTER(ctypes.c_uint64), f32p, sz, ctypes.c_double, ctypes.c_int]
         L.wha_synth_normal.restype = ctypes.c_int
         L.wha_timing_enable.argtypes = [ctypes.c_int]
@@ -442,6 +454,239 @@ def linear_bwd_dw(dy, x, compute_bias=True, workspace=None):
         _ptr(dy), lddy, _ptr(x), ldx, _ptr(dw), _ptr(db) if db is not None else None, M, N, K,
         _ptr(workspace), ws_bytes, _stream_ptr(dy)))
     return dw, db
+
+
+# ------------------------------------------------------------------ packed sequences and paged caches
+
+WHA_F32, WHA_BF16, WHA_F16, WHA_I8 = 0, 1, 2, 3
+_dtype_codes = None
+
+
+def _dtype_code(dtype, name, cache=False):
+    """WHA_F32 .. of a torch dtype (WHA_I8 for caches only)."""
+    global _dtype_codes
+    if _dtype_codes is None:
+        torch = _torch()
+        _dtype_codes = {torch.float32: WHA_F32, torch.bfloat16: WHA_BF16, torch.float16: WHA_F16, torch.int8: WHA_I8}
+    code = _dtype_codes.get(dtype)
+    if code is None or (code == WHA_I8 and not cache):
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16{' or int8' if cache else ''}, got {dtype}")
+    return code
+
+
+def _heads_layout(t, name, like=None, rows=True) -> WaveLayout:
+    """Layout of a [rows][heads][D] device view (or, rows=False, of one row of
+    heads per sequence, [B][heads][D]) with unit stride on D; `like`: the tensor
+    whose type and device it has to have."""
+    if t.dim() != 3:
+        raise ValueError(f"{name}: expected a 3-D [rows][heads][head_dim] tensor, got shape {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a device (cuda/hip) tensor")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise TypeError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    (N, H, D), (st, sh, sd) = t.shape, t.stride()
+    if sd != 1 and D > 1:
+        raise ValueError(f"{name}: the head dimension must have unit stride")
+    if H == 1:
+        sh = D
+    if N == 1:
+        st = H * sh if sh >= D else H * D
+    return WaveLayout(1, H, N, D, 0, sh, st) if rows else WaveLayout(N, H, 1, D, st, sh, H * D)
+
+
+def _index_tensor(t, name, dtype, device, dim=1):
+    if t.dtype != dtype or t.device != device or t.dim() != dim or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: expected a {dim}-D {dtype} tensor with contiguous rows on {device}, "
+                         f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _on_device(t):
+    """Kernels are launched with the tensors' device current, whichever is."""
+    torch = _torch()
+    import contextlib
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _lse_out(lse, shape, device):
+    torch = _torch()
+    if lse is None:
+        return torch.empty(shape, dtype=torch.float32, device=device)
+    if tuple(lse.shape) != shape or lse.dtype != torch.float32 or lse.device != device or not lse.is_contiguous():
+        raise ValueError(f"lse: expected a contiguous float32 {shape} tensor on {device}")
+    return lse
+
+
+def _workspace(workspace, need, device):
+    """(tensor, bytes) of a call's workspace: the caller's, or one from torch's
+    allocator (safe under stream capture, unlike the library's cached one)."""
+    torch = _torch()
+    if workspace is None:
+        return (torch.empty(need, dtype=torch.uint8, device=device), need) if need else (None, 0)
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace: expected a contiguous tensor on {device}")
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def _packed_views(q, k, v, cu_seqlens):
+    torch = _torch()
+    Lq, Lk, Lv = _heads_layout(q, "q"), _heads_layout(k, "k", q), _heads_layout(v, "v", q)
+    _index_tensor(cu_seqlens, "cu_seqlens", torch.int32, q.device)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    return Lq, Lk, Lv, cu_seqlens.numel() - 1
+
+
+def packed_fwd(q, k, v, cu_seqlens, scale=None, want_lse=True, out=None, lse=None):
+    """Causal attention of packed sequences with grouped heads (wha_packed_fwd): q
+    [N][H][D], k and v [N][Hkv][D] views (float32, bfloat16 or float16; columns of
+    a fused projection's rows as they are), cu_seqlens int32 [n_seq + 1] on the
+    device.  Returns (o, lse) with lse [H][N], or o alone when want_lse=False.
+    Rows behind the last sequence are left as they were (in a new o and lse:
+    whatever the allocator gave)."""
+    torch = _torch()
+    Lq, Lk, Lv, n_seq = _packed_views(q, k, v, cu_seqlens)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out: expected shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    Lo = _heads_layout(out, "out", q)
+    code = _dtype_code(q.dtype, "q")
+    lse = _lse_out(lse, (Lq.H, Lq.T), q.device) if want_lse else None
+    if q.numel() and n_seq > 0:
+        s = default_scale(Lq.D) if scale is None else float(scale)
+        with _on_device(q):
+            _check("wha_packed_fwd", lib().wha_packed_fwd(
+                _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cu_seqlens), n_seq, code, ctypes.byref(Lq),
+                ctypes.byref(Lk), ctypes.byref(Lv), ctypes.byref(Lo), s, _stream_ptr(q)))
+    return (out, lse) if want_lse else out
+
+
+def packed_bwd(q, k, v, o, do, lse, cu_seqlens, scale=None, workspace=None, dq=None, dk=None, dv=None):
+    """Backward of packed_fwd from its o and lse (wha_packed_bwd).  Returns (dq, dk,
+    dv), which have the strides of q, k and v (given ones too: slices of a fused
+    gradient where q, k and v are slices); do has those of o.  float32 and
+    bfloat16."""
+    torch = _torch()
+    Lq, Lk, Lv, n_seq = _packed_views(q, k, v, cu_seqlens)
+    Lo = _heads_layout(o, "o", q)
+    grads = []
+    for t, g, name in ((q, dq, "dq"), (k, dk, "dk"), (v, dv, "dv"), (o, do, "do")):
+        if g is None:
+            g = torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
+        elif g.shape != t.shape or any(n > 1 and a != b for n, a, b in zip(t.shape, g.stride(), t.stride())):
+            raise ValueError(f"{name} must have the shape and strides of {name[1:]}: {tuple(t.shape)} {t.stride()}, "
+                             f"got {tuple(g.shape)} {g.stride()}")
+        _heads_layout(g, name, q)
+        grads.append(g)
+    if o.shape != q.shape:
+        raise ValueError(f"o: expected shape {tuple(q.shape)}, got {tuple(o.shape)}")
+    code = _dtype_code(q.dtype, "q")
+    lse = _lse_out(lse, (Lq.H, Lq.T), q.device)
+    dq, dk, dv, do = grads
+    if q.numel() and n_seq > 0:
+        s = default_scale(Lq.D) if scale is None else float(scale)
+        with _on_device(q):
+            ws, ws_bytes = _workspace(workspace, int(lib().wha_packed_bwd_workspace_size(ctypes.byref(Lq))), q.device)
+            _check("wha_packed_bwd", lib().wha_packed_bwd(
+                _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(do), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
+                _ptr(cu_seqlens), n_seq, code, _ptr(ws), ws_bytes, ctypes.byref(Lq), ctypes.byref(Lk),
+                ctypes.byref(Lv), ctypes.byref(Lo), s, _stream_ptr(q)))
+    return dq, dk, dv
+
+
+def _cache_args(k_cache, v_cache, k_scale, v_scale, device):
+    """Type code, pages, heads, page size and head dim of a paged cache."""
+    torch = _torch()
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError("k_cache and v_cache must be [n_pages][n_kv_head][page_size][head_dim] tensors of one type")
+    for t in (k_cache, v_cache):
+        if t.device != device or not t.is_contiguous():
+            raise ValueError(f"k_cache and v_cache must be contiguous on {device}")
+    code = _dtype_code(k_cache.dtype, "k_cache", cache=True)
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if (t is None) != (code != WHA_I8):
+            raise ValueError(f"{name}: int8 caches have scales, others none")
+        if t is not None and (t.shape != k_cache.shape[:3] or t.dtype != torch.float32 or t.device != device
+                              or not t.is_contiguous()):
+            raise ValueError(f"{name}: expected a contiguous float32 {tuple(k_cache.shape[:3])} tensor on {device}")
+    return (code,) + tuple(k_cache.shape)
+
+
+def _paged_rows(k, v, slots, k_cache, v_cache, k_scale, v_scale):
+    torch = _torch()
+    Lk, Lv = _heads_layout(k, "k"), _heads_layout(v, "v", k)
+    ccode, pages, HK, P, D = _cache_args(k_cache, v_cache, k_scale, v_scale, k.device)
+    _index_tensor(slots, "slots", torch.int64, k.device)
+    if k.shape != v.shape or tuple(k.shape[1:]) != (HK, D) or slots.numel() != k.shape[0]:
+        raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} and {slots.numel()} slots do not belong to a cache "
+                         f"of {HK} heads of {D}")
+    return Lk, Lv, _dtype_code(k.dtype, "k"), ccode, pages, P
+
+
+def paged_kv_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
+    """Rows k and v [N][Hkv][D] into the slots (int64 [N] on the device; page *
+    page_size + place; negative: left out) of a paged cache
+    [n_pages][Hkv][page_size][D] of their type, or of int8 with scales
+    [n_pages][Hkv][page_size] (wha_paged_kv_write)."""
+    Lk, Lv, code, ccode, pages, P = _paged_rows(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    if k.numel() and pages:
+        with _on_device(k):
+            _check("wha_paged_kv_write", lib().wha_paged_kv_write(
+                _ptr(k), _ptr(v), _ptr(slots), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), code,
+                ccode, pages, P, ctypes.byref(Lk), ctypes.byref(Lv), _stream_ptr(k)))
+
+
+def paged_kv_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=None, out=None):
+    """The rows of the slots out of a paged cache again (wha_paged_kv_read): (k, v)
+    [N][Hkv][D] of `dtype` (the cache's own; for an int8 cache float32 unless
+    given), zeros for negative slots.  out: a pair of views to write to."""
+    torch = _torch()
+    if out is None:
+        if dtype is None:
+            dtype = torch.float32 if k_cache.dtype == torch.int8 else k_cache.dtype
+        shape = (slots.numel(), k_cache.shape[1], k_cache.shape[3])
+        out = tuple(torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
+    k, v = out
+    Lk, Lv, code, ccode, pages, P = _paged_rows(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    if k.numel():
+        with _on_device(k):
+            _check("wha_paged_kv_read", lib().wha_paged_kv_read(
+                _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(slots), _ptr(k), _ptr(v), code,
+                ccode, pages, P, ctypes.byref(Lk), ctypes.byref(Lv), _stream_ptr(k)))
+    return k, v
+
+
+def paged_decode_fwd(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_scale=None, scale=None,
+                     want_lse=False, workspace=None, out=None, lse=None):
+    """One query per sequence, q [B][H][D], over the first lengths[b] positions of
+    the paged cache that block_table[b] names (int32 [B][max_pages] and [B] on the
+    device; wha_paged_decode).  Returns o [B][H][D], with want_lse also lse [B][H]."""
+    torch = _torch()
+    Lq = _heads_layout(q, "q", rows=False)
+    ccode, pages, HK, P, D = _cache_args(k_cache, v_cache, k_scale, v_scale, q.device)
+    _index_tensor(block_table, "block_table", torch.int32, q.device, 2)
+    _index_tensor(lengths, "lengths", torch.int32, q.device)
+    if D != Lq.D or block_table.shape[0] != Lq.B or lengths.numel() != Lq.B:
+        raise ValueError(f"q {tuple(q.shape)}, a table of {tuple(block_table.shape)}, {lengths.numel()} lengths and a "
+                         f"cache of head dim {D} do not belong together")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out: expected shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    Lo = _heads_layout(out, "out", q, rows=False)
+    code = _dtype_code(q.dtype, "q")
+    lse = _lse_out(lse, (Lq.B, Lq.H), q.device) if want_lse else None
+    if q.numel():
+        s = default_scale(D) if scale is None else float(scale)
+        per = block_table.shape[1]
+        with _on_device(q):
+            ws, ws_bytes = _workspace(workspace, int(lib().wha_paged_decode_workspace_size(
+                ctypes.byref(Lq), HK, P, per)), q.device)
+            _check("wha_paged_decode", lib().wha_paged_decode(
+                _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_table),
+                block_table.stride(0), per, _ptr(lengths), _ptr(out), _ptr(lse), _ptr(ws), ws_bytes, code, ccode,
+                pages, P, HK, ctypes.byref(Lq), ctypes.byref(Lo), s, _stream_ptr(q)))
+    return (out, lse) if want_lse else out
 
 
 class AttnPlan:

@@ -1,0 +1,563 @@
+// Causal attention of packed sequences with grouped heads, forward and backward
+// (gfx950): sequences of any lengths one after the other in [total][heads][D]
+// rows, cu[i] .. cu[i + 1] - 1 the rows of sequence i (on the device), G query
+// heads to a key-value head.
+//
+//   s_ij = scale q_i . k_j (j <= i, same sequence), lse_i = log sum_j exp s_ij,
+//   o_i = sum_j exp(s_ij - lse_i) v_j
+//   Delta_i = do_i . o_i, p = exp(s - lse), dp_ij = do_i . v_j, ds = p (dp - Delta)
+//   dq_i = scale sum_j ds_ij k_j, dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij do_i
+//   (i over the rows of all G heads of the group)
+//
+// The G query heads of a group are rows of one matrix: row r = t G + g is
+// position t of head g, key j is before it iff j G <= r.  A block then holds
+// 128 / G positions of all of them, so its tiles past the diagonal are few also
+// for short sequences, and the key-stationary kernel sums the group as it goes.
+//
+// Scores are formed transposed where queries are kept (S^T = K Q^T: keys on MFMA
+// rows, a wave's 32 queries on columns), so that P^T is the other operand of O^T
+// += V^T P^T as it stands; with keys kept (dK, dV) as S = Q K^T, for the same
+// reason.
+#include <hip/hip_runtime.h>
+
+#include "wha_elem.hpp"
+#include "wha_packed.hpp"
+
+namespace wha {
+
+namespace {
+
+// Which tile of which sequence a block takes.  Sequence i has the slots from
+// floor(rows before it / BM) + i on, which is at least as many as it has tiles;
+// the others stay empty.  So the grid needs the total only, and a block finds its
+// sequence by comparing against 64 starts at a time.
+struct Place {
+  int tile, start, len;  // tile < 0: an empty slot
+};
+__device__ __forceinline__ int seq_start(const int* cu, int i, int total) { return min(max(cu[i], 0), total); }
+__device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total, int G, int BM, int slot, int lane) {
+  int lo = 0, n = n_seq;
+  while (n > 1) {  // at most 6 rounds: n shrinks 64-fold
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    bool before = false;
+    if (lane * step < n) before = (int)((int64_t)seq_start(cu, i, total) * G / BM) + i <= slot;
+    const int c = max(1, (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(before))) - 1;
+    lo += c * step;
+    n = min(step, n - c * step);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  Place p;
+  p.start = __builtin_amdgcn_readfirstlane(seq_start(cu, lo, total));
+  p.len = __builtin_amdgcn_readfirstlane(max(0, seq_start(cu, lo + 1, total) - p.start));
+  p.tile = slot - (int)((int64_t)p.start * G / BM) - lo;
+  if ((int64_t)p.tile * BM >= (int64_t)p.len * G) p.tile = -1;
+  return p;
+}
+
+// Rows of a tile into LDS, ROWS x DP by NT threads: row(rr) is the address of
+// tile row rr.  VEC: direct-to-LDS loads, complete after wait_vmem; quads past
+// the head dim come from 16 zero bytes.
+template <class T, int DP, int ROWS, int NT, bool VEC, class Row>
+__device__ __forceinline__ void stage(char* lds, int D, int tid, Row&& row) {
+  using L = LdsTile<T, DP>;
+  constexpr int PER = ROWS * L::kQuads / NT, Q = Elem<T>::kQuad;
+  static_assert(ROWS * L::kQuads % NT == 0, "whole rounds");
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int idx = p * NT + tid, rr = idx / L::kQuads, c = (idx % L::kQuads) ^ L::swz(rr);
+    const T* src = row(rr) + c * Q;
+    if constexpr (VEC) {
+      const float* s = c * Q < D ? reinterpret_cast<const float*>(src) : g_zero_quad;
+      dma_quad(s, reinterpret_cast<float*>(lds + (p * NT + (tid & ~63)) * 16));
+    } else {
+      T x[Q];
+#pragma unroll
+      for (int e = 0; e < Q; ++e) x[e] = c * Q + e < D ? src[e] : (T)0.f;
+      uintx4 y;
+      __builtin_memcpy(&y, x, 16);
+      *reinterpret_cast<uintx4*>(lds + idx * 16) = y;
+    }
+  }
+}
+
+// d = 16 ks + 8 g .. + 7 of one row as a fragment (zero past the head dim).
+template <class T, bool VEC>
+__device__ __forceinline__ typename Elem<T>::Frag row_frag(const T* row, int ks, int g, int D) {
+  const int c = 16 * ks + 8 * g;
+  float x[8];
+  if constexpr (VEC && sizeof(T) == 2) {
+    uintx4 q = {0u, 0u, 0u, 0u};
+    if (c < D) q = *reinterpret_cast<const uintx4*>(row + c);
+    return __builtin_bit_cast(typename Elem<T>::Frag, q);
+  } else if constexpr (VEC) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      floatx4 q = {0.f, 0.f, 0.f, 0.f};
+      if (c + 4 * h < D) q = *reinterpret_cast<const floatx4*>(row + c + 4 * h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * h + e] = q[e];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = c + j < D ? (float)row[c + j] : 0.f;
+  }
+  return Elem<T>::pack(x);
+}
+
+// Writes a lane's part of X^T[d][row] (d = 32 dt + row32(i, g)) to its row.
+template <class T, int NDT, bool VEC>
+__device__ __forceinline__ void store_row(T* dst, int D, int g, const floatx16 (&x)[NDT], float mul) {
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int c = 32 * dt + 8 * u + 4 * g;
+      if constexpr (VEC) {
+        if (c < D)
+          Elem<T>::store4(dst + c, x[dt][4 * u] * mul, x[dt][4 * u + 1] * mul, x[dt][4 * u + 2] * mul,
+                          x[dt][4 * u + 3] * mul);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < D) dst[c + e] = (T)(x[dt][4 * u + e] * mul);
+      }
+    }
+}
+
+// Whether a tile holds an infinity or NaN (one wave looks at all of it).
+template <class T, int DP, int ROWS>
+__device__ __forceinline__ bool tile_not_finite(const char* t, int lane) {
+  bool bad = false;
+#pragma unroll 4
+  for (int i = lane; i < ROWS * LdsTile<T, DP>::kQuads; i += 64)
+    bad |= quad_not_finite<T>(*reinterpret_cast<const uintx4*>(t + 16 * i));
+  return __builtin_amdgcn_ballot_w64(bad) != 0;
+}
+
+// acc[d][column] += sum over the tile's rows that belong to the column of
+// p[row][column] x[row][d].  As an MFMA wherever a weight of zero times x is
+// zero; where the mask cuts through the tile and x holds an infinity or NaN (0 x
+// inf), row by row over the rows the mask leaves.
+template <class T, int DP, int NDT, int NSUB, class Mine>
+__device__ __forceinline__ void add_rows(const char* t, const floatx16 (&p)[NSUB], floatx16 (&acc)[NDT], int lane,
+                                         Mine&& mine) {
+  const int g = lane >> 5, c = lane & 31;
+#pragma unroll 1
+  for (int x = 0; x < 32 * NSUB; ++x) {
+    const int i = 4 * ((x & 31) >> 3) + (x & 3), h = (x >> 2) & 1;
+    float px = 0.f;
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) px = s == (x >> 5) && j == i ? p[s][j] : px;
+    px = __shfl(px, c + 32 * h, 64);
+    if (mine(x)) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int y = 0; y < 16; ++y)
+          acc[dt][y] = fmaf(px, LdsTile<T, DP>::one(t, x, 32 * dt + row32(y, g)), acc[dt][y]);
+    }
+  }
+}
+template <class T, int DP, int NDT, int NSUB>
+__device__ __forceinline__ void add_cols(const char* t, const floatx16 (&p)[NSUB], floatx16 (&acc)[NDT], int lane) {
+#pragma unroll
+  for (int s = 0; s < NSUB; ++s)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = p[s][8 * h + j];
+      const typename Elem<T>::Frag f = Elem<T>::pack(x);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+        acc[dt] = Elem<T>::mma32(LdsTile<T, DP>::cols32(t, 2 * s + h, dt, lane), f, acc[dt]);
+    }
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------- forward
+template <class T, int NKS, int NDT, bool VEC>
+__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+                                                            const T* __restrict__ V, T* __restrict__ O,
+                                                            float* __restrict__ LSE, PackedArgs a, float sl2) {
+  constexpr int DP = 32 * NDT, NT = 256, BM = 128, KT = sizeof(T) == 4 ? 32 : 64, NSUB = KT / 32;
+  using L = LdsTile<T, DP>;
+  constexpr int BYTES = KT * L::kRow;
+  __shared__ __align__(16) char K0[BYTES], K1[BYTES], V0[BYTES], V1[BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // a key-value head's blocks share an XCD's L2 where there are 8 of them; the
+  // later tiles of a sequence, which sweep more keys, first
+  const int hk = blockIdx.x % a.HK, slot = a.slots - 1 - (int)(blockIdx.x / a.HK);
+  const Place pl = find_place(a.cu, a.n_seq, a.total, G, BM, slot, lane);
+  if (pl.tile < 0) return;
+  const int rows = pl.len * G, r0 = pl.tile * BM + wave * 32;
+  const int r = r0 + (lane & 31), rc = min(r, rows - 1), t = rc / G, h = hk * G + rc % G;
+  const T* Kb = K + (int64_t)pl.start * a.k_st + (int64_t)hk * a.k_sh;
+  const T* Vb = V + (int64_t)pl.start * a.v_st + (int64_t)hk * a.v_sh;
+  auto stage_kv = [&](int kt, char* Kd, char* Vd) {
+    stage<T, DP, KT, NT, VEC>(Kd, D, tid, [&](int rr) { return Kb + (int64_t)min(kt * KT + rr, pl.len - 1) * a.k_st; });
+    stage<T, DP, KT, NT, VEC>(Vd, D, tid, [&](int rr) { return Vb + (int64_t)min(kt * KT + rr, pl.len - 1) * a.v_st; });
+  };
+  const int n_kt = min(pl.tile * BM + BM - 1, rows - 1) / G / KT + 1;  // tiles that the block sweeps
+  const int t_first = __builtin_amdgcn_readfirstlane(t), t_last = __builtin_amdgcn_readlane(t, 31);
+  const int n_w = r0 < rows ? t_last / KT + 1 : 0;  // tiles with a key before some query of the wave
+  stage_kv(0, K0, V0);
+
+  typename Elem<T>::Frag qf[NKS];
+  const T* Qr = Q + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) qf[ks] = row_frag<T, VEC>(Qr, ks, g, D);
+
+  float m = -INFINITY, l = 0.f;  // running maximum (log2 units), this lane's part of the row sum
+  floatx16 o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) o[dt] = zeros16();
+
+  auto tile = [&](int kt, const char* Kt, const char* Vt) {
+    const int k0 = kt * KT;
+    floatx16 s[NSUB];
+#pragma unroll
+    for (int x = 0; x < NSUB; ++x) {
+      s[x] = zeros16();
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks)
+        s[x] = Elem<T>::mma32(L::rows32(Kt, 32 * x + (lane & 31), ks, g), qf[ks], s[x]);
+    }
+    const bool cut = k0 + KT - 1 > t_first;  // wave-uniform: the mask cuts through the tile
+    if (cut) {
+#pragma unroll
+      for (int x = 0; x < NSUB; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] = k0 + 32 * x + row32(i, g) > t ? -INFINITY : s[x][i];
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int x = 0; x < NSUB; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = vmax2(mx, s[x][i]);
+    mx = pair_max32(mx) * sl2;
+    // O and l keep the maximum they have until one passes it by 2^8: the sums
+    // stay far from fp32's and P from its type's limits, and most tiles need no
+    // rescaling
+    if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
+      const float mn = vmax2(m, mx), alpha = mn == m ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+    }
+    const float sub = m == -INFINITY ? 0.f : m;  // only scores of -inf so far: weights of 0
+#pragma unroll
+    for (int x = 0; x < NSUB; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[x][i] = fast_exp2(fmaf(s[x][i], sl2, -sub));
+        l += s[x][i];
+      }
+    if (cut && tile_not_finite<T, DP, KT>(Vt, lane))
+      add_rows<T, DP>(Vt, s, o, lane, [&](int x) { return k0 + x <= t; });
+    else
+      add_cols<T, DP>(Vt, s, o, lane);
+  };
+  auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
+    if constexpr (VEC) wait_vmem();
+    __syncthreads();  // tile kt is in LDS; every wave is done with the other buffers
+    if (kt + 1 < n_kt) stage_kv(kt + 1, Kn, Vn);
+    if (kt < n_w) tile(kt, Kt, Vt);
+  };
+  for (int kt = 0; kt < n_kt; kt += 2) {
+    step(kt, K0, V0, K1, V1);
+    if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
+  }
+  l = pair_sum32(l);
+  if (r < rows) {
+    store_row<T, NDT, VEC>(O + (int64_t)(pl.start + t) * a.o_st + (int64_t)h * a.o_sh, D, g, o, 1.f / l);
+    if (LSE != nullptr && g == 0) LSE[(int64_t)h * a.total + pl.start + t] = fmaf(m, kLn2, logf(l));
+  }
+}
+
+// ---------------------------------------------------------------- backward
+// Query-stationary: dQ, and the row statistics lse log2(e) and Delta that the
+// key-stationary kernel reads.
+template <class T, int NKS, int NDT, bool VEC>
+__global__ __launch_bounds__(256, 2) void packed_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+                                                           const T* __restrict__ V, const T* __restrict__ O,
+                                                           const T* __restrict__ DO, const float* __restrict__ LSE,
+                                                           T* __restrict__ DQ, float* __restrict__ LSE2,
+                                                           float* __restrict__ DELTA, PackedArgs a, float sl2,
+                                                           float scale) {
+  constexpr int DP = 32 * NDT, NT = 256, BM = 128, KT = sizeof(T) == 4 ? 32 : 64, NSUB = KT / 32;
+  using L = LdsTile<T, DP>;
+  constexpr int BYTES = KT * L::kRow;
+  __shared__ __align__(16) char K0[BYTES], K1[BYTES], V0[BYTES], V1[BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hk = blockIdx.x % a.HK, slot = a.slots - 1 - (int)(blockIdx.x / a.HK);
+  const Place pl = find_place(a.cu, a.n_seq, a.total, G, BM, slot, lane);
+  if (pl.tile < 0) return;
+  const int rows = pl.len * G, r0 = pl.tile * BM + wave * 32;
+  const int r = r0 + (lane & 31), rc = min(r, rows - 1), t = rc / G, h = hk * G + rc % G;
+  const T* Kb = K + (int64_t)pl.start * a.k_st + (int64_t)hk * a.k_sh;
+  const T* Vb = V + (int64_t)pl.start * a.v_st + (int64_t)hk * a.v_sh;
+  auto stage_kv = [&](int kt, char* Kd, char* Vd) {
+    stage<T, DP, KT, NT, VEC>(Kd, D, tid, [&](int rr) { return Kb + (int64_t)min(kt * KT + rr, pl.len - 1) * a.k_st; });
+    stage<T, DP, KT, NT, VEC>(Vd, D, tid, [&](int rr) { return Vb + (int64_t)min(kt * KT + rr, pl.len - 1) * a.v_st; });
+  };
+  const int n_kt = min(pl.tile * BM + BM - 1, rows - 1) / G / KT + 1;
+  const int t_first = __builtin_amdgcn_readfirstlane(t), t_last = __builtin_amdgcn_readlane(t, 31);
+  const int n_w = r0 < rows ? t_last / KT + 1 : 0;
+  stage_kv(0, K0, V0);
+
+  typename Elem<T>::Frag qf[NKS], dof[NKS];
+  const T* Qr = Q + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh;
+  const int64_t o_at = (int64_t)(pl.start + t) * a.o_st + (int64_t)h * a.o_sh;
+  const int64_t stat_at = (int64_t)h * a.total + pl.start + t;
+  float delta = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    qf[ks] = row_frag<T, VEC>(Qr, ks, g, D);
+    dof[ks] = row_frag<T, VEC>(DO + o_at, ks, g, D);
+    const typename Elem<T>::Frag of = row_frag<T, VEC>(O + o_at, ks, g, D);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) delta = fmaf((float)of[j], (float)dof[ks][j], delta);
+  }
+  delta = pair_sum32(delta);
+  const float lse2 = LSE[stat_at] * kLog2e;
+  if (r < rows && g == 0) {
+    LSE2[stat_at] = lse2;
+    DELTA[stat_at] = delta;
+  }
+  floatx16 dq[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dq[dt] = zeros16();
+
+  auto tile = [&](int kt, const char* Kt, const char* Vt) {
+    const int k0 = kt * KT;
+    floatx16 ds[NSUB];
+    const bool cut = k0 + KT - 1 > t_first;
+#pragma unroll
+    for (int x = 0; x < NSUB; ++x) {
+      floatx16 s = zeros16(), dp = zeros16();
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        s = Elem<T>::mma32(L::rows32(Kt, 32 * x + (lane & 31), ks, g), qf[ks], s);
+        dp = Elem<T>::mma32(L::rows32(Vt, 32 * x + (lane & 31), ks, g), dof[ks], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[x][i] = fast_exp2(fmaf(s[i], sl2, -lse2)) * (dp[i] - delta);
+      if (cut) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[x][i] = k0 + 32 * x + row32(i, g) > t ? 0.f : ds[x][i];
+      }
+    }
+    if (cut && tile_not_finite<T, DP, KT>(Kt, lane))
+      add_rows<T, DP>(Kt, ds, dq, lane, [&](int x) { return k0 + x <= t; });
+    else
+      add_cols<T, DP>(Kt, ds, dq, lane);
+  };
+  auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
+    if constexpr (VEC) wait_vmem();
+    __syncthreads();
+    if (kt + 1 < n_kt) stage_kv(kt + 1, Kn, Vn);
+    if (kt < n_w) tile(kt, Kt, Vt);
+  };
+  for (int kt = 0; kt < n_kt; kt += 2) {
+    step(kt, K0, V0, K1, V1);
+    if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
+  }
+  if (r < rows)
+    store_row<T, NDT, VEC>(DQ + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh, D, g, dq, scale);
+}
+
+// Key-stationary: dK and dV of 128 keys, over the rows of the group that come
+// after them.
+template <class T, int NKS, int NDT, bool VEC>
+__global__ __launch_bounds__(256, 2) void packed_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+                                                            const T* __restrict__ V, const T* __restrict__ DO,
+                                                            const float* __restrict__ LSE2,
+                                                            const float* __restrict__ DELTA, T* __restrict__ DK,
+                                                            T* __restrict__ DV, PackedArgs a, float sl2, float scale) {
+  constexpr int DP = 32 * NDT, NT = 256, BN = 128, QT = 32;
+  using L = LdsTile<T, DP>;
+  constexpr int BYTES = QT * L::kRow;
+  __shared__ __align__(16) char Q0[BYTES], Q1[BYTES], D0[BYTES], D1[BYTES];
+  __shared__ __align__(16) float S0[64], S1[64];  // a tile's lse log2(e), then its Delta
+
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // the earlier keys of a sequence, which more rows come after, first
+  const int hk = blockIdx.x % a.HK, slot = (int)(blockIdx.x / a.HK);
+  const Place pl = find_place(a.cu, a.n_seq, a.total, 1, BN, slot, lane);
+  if (pl.tile < 0) return;
+  const int rows = pl.len * G, key0 = pl.tile * BN + wave * 32;
+  const int key = key0 + (lane & 31), kc = min(key, pl.len - 1);
+  const int first = key * G;  // the first row that comes at or after the key
+  const T* Qb = Q + (int64_t)pl.start * a.q_st + (int64_t)hk * G * a.q_sh;
+  const T* Db = DO + (int64_t)pl.start * a.o_st + (int64_t)hk * G * a.o_sh;
+  const int64_t stat0 = (int64_t)hk * G * a.total + pl.start;
+  // position and head of a tile's row (G <= 128: a 16-bit reciprocal is exact
+  // below 512)
+  const int magic = 65535 / G + 1;
+  auto stage_q = [&](int rt, char* Qd, char* Dd, float* Sd) {
+    const int t0 = rt * QT / G, g0 = rt * QT % G;
+    auto place = [&](int rr, int& t, int& gq) {
+      const int x = min(rr, rows - 1 - rt * QT) + g0, y = (x * magic) >> 16;
+      t = t0 + y;
+      gq = x - y * G;
+    };
+    stage<T, DP, QT, NT, VEC>(Qd, D, tid, [&](int rr) {
+      int t, gq;
+      place(rr, t, gq);
+      return Qb + (int64_t)t * a.q_st + (int64_t)gq * a.q_sh;
+    });
+    stage<T, DP, QT, NT, VEC>(Dd, D, tid, [&](int rr) {
+      int t, gq;
+      place(rr, t, gq);
+      return Db + (int64_t)t * a.o_st + (int64_t)gq * a.o_sh;
+    });
+    if (wave == 0) {
+      int t, gq;
+      place(lane & 31, t, gq);
+      const int64_t at = stat0 + (int64_t)gq * a.total + t;
+      dma_dword(lane < 32 ? LSE2 + at : DELTA + at, Sd);
+    }
+  };
+  const int rt0 = pl.tile * BN * G / QT, n_rt = (rows + QT - 1) / QT;
+  const int rt_w = key0 < pl.len ? key0 * G / QT : n_rt;  // the first tile with a row after some key of the wave
+  stage_q(rt0, Q0, D0, S0);
+
+  typename Elem<T>::Frag kf[NKS], vf[NKS];
+  const T* Kr = K + (int64_t)(pl.start + kc) * a.k_st + (int64_t)hk * a.k_sh;
+  const T* Vr = V + (int64_t)(pl.start + kc) * a.v_st + (int64_t)hk * a.v_sh;
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    kf[ks] = row_frag<T, VEC>(Kr, ks, g, D);
+    vf[ks] = row_frag<T, VEC>(Vr, ks, g, D);
+  }
+  floatx16 dk[NDT], dv[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dk[dt] = zeros16(), dv[dt] = zeros16();
+
+  auto tile = [&](int rt, const char* Qt, const char* Dt, const float* St) {
+    const int r0 = rt * QT;
+    floatx16 p[1], ds[1];
+    floatx16 s = zeros16(), dp = zeros16();
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      s = Elem<T>::mma32(L::rows32(Qt, lane & 31, ks, g), kf[ks], s);
+      dp = Elem<T>::mma32(L::rows32(Dt, lane & 31, ks, g), vf[ks], dp);
+    }
+    // the mask (or the sequence's end) cuts through the tile
+    const bool cut = r0 < (key0 + 31) * G || r0 + QT > rows;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const floatx4 lse2 = *reinterpret_cast<const floatx4*>(St + 8 * u + 4 * g);
+      const floatx4 delta = *reinterpret_cast<const floatx4*>(St + 32 + 8 * u + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * u + e;
+        p[0][i] = fast_exp2(fmaf(s[i], sl2, -lse2[e]));
+        ds[0][i] = p[0][i] * (dp[i] - delta[e]);
+      }
+    }
+    auto mine = [&](int x) { return r0 + x >= first && r0 + x < rows; };
+    if (cut) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool in = mine(row32(i, g));
+        p[0][i] = in ? p[0][i] : 0.f;
+        ds[0][i] = in ? ds[0][i] : 0.f;
+      }
+    }
+    if (cut && (tile_not_finite<T, DP, QT>(Qt, lane) || tile_not_finite<T, DP, QT>(Dt, lane))) {
+      add_rows<T, DP>(Dt, p, dv, lane, mine);
+      add_rows<T, DP>(Qt, ds, dk, lane, mine);
+    } else {
+      add_cols<T, DP>(Dt, p, dv, lane);
+      add_cols<T, DP>(Qt, ds, dk, lane);
+    }
+  };
+  auto step = [&](int rt, char* Qt, char* Dt, float* St, char* Qn, char* Dn, float* Sn) {
+    wait_vmem();
+    __syncthreads();
+    if (rt + 1 < n_rt) stage_q(rt + 1, Qn, Dn, Sn);
+    if (rt >= rt_w) tile(rt, Qt, Dt, St);
+  };
+  for (int rt = rt0; rt < n_rt; rt += 2) {
+    step(rt, Q0, D0, S0, Q1, D1, S1);
+    if (rt + 1 < n_rt) step(rt + 1, Q1, D1, S1, Q0, D0, S0);
+  }
+  if (key < pl.len) {
+    store_row<T, NDT, VEC>(DK + (int64_t)(pl.start + key) * a.k_st + (int64_t)hk * a.k_sh, D, g, dk, scale);
+    store_row<T, NDT, VEC>(DV + (int64_t)(pl.start + key) * a.v_st + (int64_t)hk * a.v_sh, D, g, dv, 1.f);
+  }
+}
+
+// ---------------------------------------------------------------- launches
+namespace {
+
+template <class T, int NKS, int NDT, bool VEC>
+hipError_t fwd_t(const void* q, const void* k, const void* v, void* o, float* lse, PackedArgs a, float scale,
+                 hipStream_t stream) {
+  a.slots = packed_slots(a, 128, a.G);
+  TimingScope ts("packed_fwd", stream);
+  hipLaunchKernelGGL((packed_fwd_kernel<T, NKS, NDT, VEC>), dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream,
+                     static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                     static_cast<T*>(o), lse, a, (float)((double)scale * 1.4426950408889634));
+  return hipGetLastError();
+}
+
+template <class T, int NKS, int NDT, bool VEC>
+hipError_t bwd_t(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+                 void* dq, void* dk, void* dv, float* ws, PackedArgs a, float scale, hipStream_t stream) {
+  const float sl2 = (float)((double)scale * 1.4426950408889634);
+  float *lse2 = ws, *delta = ws + (int64_t)a.total * a.HK * a.G;
+  {
+    TimingScope ts("packed_bwd_dq", stream);
+    a.slots = packed_slots(a, 128, a.G);
+    hipLaunchKernelGGL((packed_dq_kernel<T, NKS, NDT, VEC>), dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream,
+                       static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                       static_cast<const T*>(o), static_cast<const T*>(d_o), lse, static_cast<T*>(dq), lse2, delta, a,
+                       sl2, scale);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  TimingScope ts("packed_bwd_dkv", stream);
+  a.slots = packed_slots(a, 128, 1);
+  hipLaunchKernelGGL((packed_dkv_kernel<T, NKS, NDT, VEC>), dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream,
+                     static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                     static_cast<const T*>(d_o), lse2, delta, static_cast<T*>(dk), static_cast<T*>(dv), a, sl2, scale);
+  return hipGetLastError();
+}
+
+// NKS: steps of 16 over the head dim, NDT: 32-wide tiles of it
+#define WHA_BY_DIM(F, T, D, vec, ...)                       \
+  (D) <= 64 ? ((vec) ? F<T, 4, 2, true>(__VA_ARGS__) : F<T, 4, 2, false>(__VA_ARGS__)) \
+            : ((vec) ? F<T, 8, 4, true>(__VA_ARGS__) : F<T, 8, 4, false>(__VA_ARGS__))
+
+}  // namespace
+
+hipError_t launch_packed_fwd(int dtype, const void* q, const void* k, const void* v, void* o, float* lse,
+                             const PackedArgs& a, bool vec, float scale, hipStream_t stream) {
+  if (dtype == kF32) return WHA_BY_DIM(fwd_t, float, a.D, vec, q, k, v, o, lse, a, scale, stream);
+  if (dtype == kBf16) return WHA_BY_DIM(fwd_t, __bf16, a.D, vec, q, k, v, o, lse, a, scale, stream);
+  return WHA_BY_DIM(fwd_t, _Float16, a.D, vec, q, k, v, o, lse, a, scale, stream);
+}
+
+hipError_t launch_packed_bwd(int dtype, const void* q, const void* k, const void* v, const void* o, const void* d_o,
+                             const float* lse, void* dq, void* dk, void* dv, float* ws, const PackedArgs& a, bool vec,
+                             float scale, hipStream_t stream) {
+  if (dtype == kF32)
+    return WHA_BY_DIM(bwd_t, float, a.D, vec, q, k, v, o, d_o, lse, dq, dk, dv, ws, a, scale, stream);
+  return WHA_BY_DIM(bwd_t, __bf16, a.D, vec, q, k, v, o, d_o, lse, dq, dk, dv, ws, a, scale, stream);
+}
+
+}  // namespace wha

@@ -16,6 +16,7 @@
 
 #include "../../include/wave_hip_attn.h"
 #include "wha_launch.hpp"
+#include "wha_packed.hpp"
 
 #ifndef WHA_VERSION
 #define WHA_VERSION "0.1.0"
@@ -1435,6 +1436,240 @@ int wha_timing_read(const char* kernel, double* total_ms, int64_t* launches) {
   *total_ms = it == st.totals.end() ? 0.0 : it->second.first;
   *launches = it == st.totals.end() ? 0 : it->second.second;
   return rc;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- packed sequences and paged caches
+namespace {
+
+// One [rows][heads][D] view (B = 1) or, with one row, [B][heads][D].
+int check_view(const wha_layout* L, const char* fn, const char* name) {
+  wha::View V;
+  const int rc = check_layout(L, &V, fn);
+  if (rc == WHA_OK) return rc;
+  const std::string why(g_err);
+  return fail(rc, "%s (%s)", why.c_str(), name);
+}
+int check_dtype(int32_t dtype, const char* fn) {
+  if (dtype != WHA_F32 && dtype != WHA_BF16 && dtype != WHA_F16)
+    return fail(WHA_ERR_INVALID, "%s: dtype %d is not WHA_F32, WHA_BF16 or WHA_F16", fn, dtype);
+  return WHA_OK;
+}
+// 16-byte loads of the rows of these views
+bool rows_aligned(size_t size, std::initializer_list<const wha_layout*> views,
+                  std::initializer_list<const void*> ptrs) {
+  const int quad = (int)(16 / size);
+  for (const wha_layout* L : views)
+    if (L->D % quad || L->stride_t % quad || L->stride_h % quad || L->stride_b % quad) return false;
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return false;
+  return true;
+}
+
+int check_packed(const char* fn, const int32_t* cu, int32_t n_seq, int32_t dtype, const wha_layout* q,
+                 const wha_layout* k, const wha_layout* v, const wha_layout* o, float scale, wha::PackedArgs* a) {
+  int rc;
+  const wha_layout* views[] = {q, k, v, o};
+  const char* names[] = {"q_layout", "k_layout", "v_layout", "o_layout"};
+  for (int i = 0; i < 4; ++i) {
+    if ((rc = check_view(views[i], fn, names[i]))) return rc;
+    if (views[i]->B != 1 || views[i]->T != q->T || views[i]->D != q->D)
+      return fail(WHA_ERR_INVALID, "%s: %s must have B = 1 and q's rows and head dim", fn, names[i]);
+  }
+  if (k->H != v->H || o->H != q->H || q->H % k->H != 0)
+    return fail(WHA_ERR_INVALID, "%s: %d / %d key / value heads for %d query heads (%d in o)", fn, k->H, v->H, q->H,
+                o->H);
+  if (q->H / k->H > 128)
+    return fail(WHA_ERR_UNSUPPORTED, "%s: more than 128 query heads to a key-value head (%d)", fn, q->H / k->H);
+  if ((rc = check_dtype(dtype, fn))) return rc;
+  if ((rc = check_scale(scale, fn))) return rc;
+  if (n_seq <= 0 || !cu) return fail(WHA_ERR_INVALID, "%s: n_seq must be positive and cu_seqlens non-NULL", fn);
+  const int G = q->H / k->H;
+  if ((int64_t)q->T * q->H >= ((int64_t)1 << 31) - (1 << 16) ||
+      wha::packed_slots64(q->T, n_seq, 128, G) * k->H >= ((int64_t)1 << 31))
+    return fail(WHA_ERR_UNSUPPORTED, "%s: rows x heads, or sequences x heads, too large", fn);
+  *a = wha::PackedArgs{cu, n_seq, q->T, k->H, G, q->D, 0, q->stride_t, q->stride_h, k->stride_t, k->stride_h,
+                       v->stride_t, v->stride_h, o->stride_t, o->stride_h};
+  return WHA_OK;
+}
+
+// Type, pages and scales of a paged cache of HK heads of D.
+int check_cache(const char* fn, const void* k, const void* v, const float* ks, const float* vs, int32_t dtype,
+                int32_t cache_dtype, int64_t n_pages, int32_t page_size, int32_t HK, int32_t D, wha::PagedCache* c) {
+  int rc;
+  if ((rc = check_dtype(dtype, fn))) return rc;
+  if (cache_dtype != dtype && cache_dtype != WHA_I8)
+    return fail(WHA_ERR_INVALID, "%s: cache_dtype %d is neither dtype (%d) nor WHA_I8", fn, cache_dtype, dtype);
+  if (!k || !v) return fail(WHA_ERR_INVALID, "%s: k_cache and v_cache must be non-NULL", fn);
+  if (cache_dtype == WHA_I8 && (!ks || !vs))
+    return fail(WHA_ERR_INVALID, "%s: an 8-bit cache needs k_scale and v_scale", fn);
+  if (page_size < 1 || page_size > 4096 || (page_size & (page_size - 1)))
+    return fail(WHA_ERR_INVALID, "%s: page_size must be a power of two up to 4096 (got %d)", fn, page_size);
+  if (n_pages < 1 || n_pages > (int64_t)1 << 31)
+    return fail(WHA_ERR_INVALID, "%s: n_pages must be in [1, 2^31] (got %lld)", fn, (long long)n_pages);
+  int shift = 0;
+  while ((1 << shift) < page_size) ++shift;
+  *c = wha::PagedCache{const_cast<void*>(k), const_cast<void*>(v), const_cast<float*>(ks), const_cast<float*>(vs),
+                       n_pages, HK, D, shift};
+  return WHA_OK;
+}
+
+int check_kv_rows(const char* fn, const void* k, const void* v, const int64_t* slots, const wha_layout* kl,
+                  const wha_layout* vl, wha::PagedRows* r) {
+  int rc;
+  if ((rc = check_view(kl, fn, "k_layout"))) return rc;
+  if ((rc = check_view(vl, fn, "v_layout"))) return rc;
+  if (kl->B != 1 || vl->B != 1 || vl->T != kl->T || vl->H != kl->H || vl->D != kl->D)
+    return fail(WHA_ERR_INVALID, "%s: k and v must have B = 1 and the same rows, heads and head dim", fn);
+  if (!k || !v || !slots) return fail(WHA_ERR_INVALID, "%s: k, v and slots must be non-NULL", fn);
+  *r = wha::PagedRows{kl->T, kl->stride_t, kl->stride_h, vl->stride_t, vl->stride_h, slots};
+  return WHA_OK;
+}
+
+bool paged_vec(const wha::PagedCache& c, size_t size, std::initializer_list<const wha_layout*> views,
+               std::initializer_list<const void*> ptrs) {
+  return c.D % 8 == 0 && aligned16(c.k) && aligned16(c.v) && rows_aligned(size, views, ptrs);
+}
+
+}  // namespace
+
+extern "C" {
+
+int wha_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_seqlens,
+                   int32_t n_seq, int32_t dtype, const wha_layout* q_layout, const wha_layout* k_layout,
+                   const wha_layout* v_layout, const wha_layout* o_layout, float scale, void* stream) {
+  static const char* fn = "wha_packed_fwd";
+  wha::PackedArgs a;
+  const int rc = check_packed(fn, cu_seqlens, n_seq, dtype, q_layout, k_layout, v_layout, o_layout, scale, &a);
+  if (rc) return rc;
+  if (!q || !k || !v || !o) return fail(WHA_ERR_INVALID, "%s: q, k, v and o must be non-NULL", fn);
+  const bool vec = rows_aligned(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout}, {q, k, v, o});
+  const hipError_t e =
+      wha::launch_packed_fwd(dtype, q, k, v, o, lse, a, vec, scale, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "wha_packed_fwd launch");
+  g_err[0] = 0;
+  return WHA_OK;
+}
+
+size_t wha_packed_bwd_workspace_size(const wha_layout* L) {
+  if (!L || L->B != 1 || L->H <= 0 || L->T <= 0) return 0;
+  return round256((size_t)L->T * L->H * 2 * sizeof(float));
+}
+
+int wha_packed_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+                   void* dq, void* dk, void* dv, const int32_t* cu_seqlens, int32_t n_seq, int32_t dtype,
+                   void* workspace, size_t workspace_bytes, const wha_layout* q_layout, const wha_layout* k_layout,
+                   const wha_layout* v_layout, const wha_layout* o_layout, float scale, void* stream) {
+  static const char* fn = "wha_packed_bwd";
+  wha::PackedArgs a;
+  int rc = check_packed(fn, cu_seqlens, n_seq, dtype, q_layout, k_layout, v_layout, o_layout, scale, &a);
+  if (rc) return rc;
+  if (dtype == WHA_F16)
+    return fail(WHA_ERR_UNSUPPORTED, "%s: no fp16 gradients (score gradients fall below its range): use WHA_BF16 "
+                "or WHA_F32", fn);
+  if (!q || !k || !v || !o || !d_o || !lse || !dq || !dk || !dv)
+    return fail(WHA_ERR_INVALID, "%s: every tensor pointer must be non-NULL", fn);
+  const bool vec = rows_aligned(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout},
+                                {q, k, v, o, d_o, dq, dk, dv});
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  void* ws = nullptr;
+  if ((rc = resolve_workspace(workspace, workspace_bytes, wha_packed_bwd_workspace_size(q_layout), s, fn, &ws)))
+    return rc;
+  const hipError_t e = wha::launch_packed_bwd(dtype, q, k, v, o, d_o, lse, dq, dk, dv, static_cast<float*>(ws), a,
+                                              vec, scale, s);
+  if (e != hipSuccess) return hip_fail(e, "wha_packed_bwd launch");
+  g_err[0] = 0;
+  return WHA_OK;
+}
+
+int wha_paged_kv_write(const void* k, const void* v, const int64_t* slots, void* k_cache, void* v_cache,
+                       float* k_scale, float* v_scale, int32_t dtype, int32_t cache_dtype, int64_t n_pages,
+                       int32_t page_size, const wha_layout* k_layout, const wha_layout* v_layout, void* stream) {
+  static const char* fn = "wha_paged_kv_write";
+  wha::PagedRows r;
+  wha::PagedCache c;
+  int rc = check_kv_rows(fn, k, v, slots, k_layout, v_layout, &r);
+  if (rc) return rc;
+  if ((rc = check_cache(fn, k_cache, v_cache, k_scale, v_scale, dtype, cache_dtype, n_pages, page_size, k_layout->H,
+                        k_layout->D, &c)))
+    return rc;
+  const bool vec = paged_vec(c, wha::elem_size(dtype), {k_layout, v_layout}, {k, v});
+  const hipError_t e =
+      wha::launch_paged_kv_write(dtype, cache_dtype, k, v, r, c, vec, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "wha_paged_kv_write launch");
+  g_err[0] = 0;
+  return WHA_OK;
+}
+
+int wha_paged_kv_read(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                      const int64_t* slots, void* k, void* v, int32_t dtype, int32_t cache_dtype, int64_t n_pages,
+                      int32_t page_size, const wha_layout* k_layout, const wha_layout* v_layout, void* stream) {
+  static const char* fn = "wha_paged_kv_read";
+  wha::PagedRows r;
+  wha::PagedCache c;
+  int rc = check_kv_rows(fn, k, v, slots, k_layout, v_layout, &r);
+  if (rc) return rc;
+  if ((rc = check_cache(fn, k_cache, v_cache, k_scale, v_scale, dtype, cache_dtype, n_pages, page_size, k_layout->H,
+                        k_layout->D, &c)))
+    return rc;
+  const bool vec = paged_vec(c, wha::elem_size(dtype), {k_layout, v_layout}, {k, v});
+  const hipError_t e =
+      wha::launch_paged_kv_read(dtype, cache_dtype, k, v, r, c, vec, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "wha_paged_kv_read launch");
+  g_err[0] = 0;
+  return WHA_OK;
+}
+
+size_t wha_paged_decode_workspace_size(const wha_layout* L, int32_t n_kv_head, int32_t page_size, int32_t max_pages) {
+  if (!L || L->B <= 0 || L->H <= 0 || L->D <= 0 || n_kv_head <= 0 || L->H % n_kv_head || page_size <= 0 ||
+      max_pages <= 0)
+    return 0;
+  return round256(sizeof(float) * wha::paged_decode_floats(L->B, L->H, n_kv_head, L->D,
+                                                           (int64_t)max_pages * page_size));
+}
+
+int wha_paged_decode(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                     const float* v_scale, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
+                     const int32_t* lengths, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                     int32_t dtype, int32_t cache_dtype, int64_t n_pages, int32_t page_size, int32_t n_kv_head,
+                     const wha_layout* q_layout, const wha_layout* o_layout, float scale, void* stream) {
+  static const char* fn = "wha_paged_decode";
+  int rc;
+  if ((rc = check_view(q_layout, fn, "q_layout"))) return rc;
+  if ((rc = check_view(o_layout, fn, "o_layout"))) return rc;
+  const wha_layout &ql = *q_layout, &ol = *o_layout;
+  if (ql.T != 1 || ol.T != 1 || ol.B != ql.B || ol.H != ql.H || ol.D != ql.D)
+    return fail(WHA_ERR_INVALID, "%s: q and o must have T = 1 and the same B, H and D", fn);
+  if (n_kv_head <= 0 || ql.H % n_kv_head)
+    return fail(WHA_ERR_INVALID, "%s: %d key-value heads for %d query heads", fn, n_kv_head, ql.H);
+  if ((rc = check_scale(scale, fn))) return rc;
+  wha::PagedCache c;
+  if ((rc = check_cache(fn, k_cache, v_cache, k_scale, v_scale, dtype, cache_dtype, n_pages, page_size, n_kv_head,
+                        ql.D, &c)))
+    return rc;
+  if (!q || !o || !block_table || !lengths)
+    return fail(WHA_ERR_INVALID, "%s: q, o, block_table and lengths must be non-NULL", fn);
+  if (max_pages <= 0 || (ql.B > 1 && table_stride < max_pages))
+    return fail(WHA_ERR_INVALID, "%s: max_pages must be positive and at most table_stride (got %d, %lld)", fn,
+                max_pages, (long long)table_stride);
+  if ((int64_t)max_pages * page_size > (int64_t)1 << 30)
+    return fail(WHA_ERR_UNSUPPORTED, "%s: more than 2^30 positions in a table's row", fn);
+  const int64_t cap = (int64_t)max_pages * page_size;
+  if ((int64_t)wha::paged_splits(ql.B, ql.H, n_kv_head, cap) * ql.B * ql.H >= (int64_t)1 << 31)
+    return fail(WHA_ERR_UNSUPPORTED, "%s: too many sequences x heads", fn);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  void* ws = nullptr;
+  const size_t need = wha_paged_decode_workspace_size(q_layout, n_kv_head, page_size, max_pages);
+  if (need && (rc = resolve_workspace(workspace, workspace_bytes, need, s, fn, &ws))) return rc;
+  const bool vec = paged_vec(c, wha::elem_size(dtype), {q_layout}, {q});
+  const wha::PagedDecode d{block_table, lengths, table_stride, ql.B, ql.H, max_pages, ql.stride_b, ql.stride_h,
+                           ol.stride_b, ol.stride_h};
+  const hipError_t e =
+      wha::launch_paged_decode(dtype, cache_dtype, q, o, lse, static_cast<float*>(ws), d, c, vec, scale, s);
+  if (e != hipSuccess) return hip_fail(e, "wha_paged_decode launch");
+  g_err[0] = 0;
+  return WHA_OK;
 }
 
 }  // extern "C"
