@@ -124,6 +124,25 @@ __device__ __forceinline__ void store_row(T* dst, int D, int g, const floatx16 (
     }
 }
 
+// N steps whose operands come from LDS: the reads of step i + 1 go out before the
+// MFMAs of step i, no more of them, so that they cost few registers.
+template <int N, class Load, class Use>
+__device__ __forceinline__ void one_ahead(Load&& load, Use&& use) {
+  auto f = load(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    auto next = f;
+    if (i + 1 < N) next = load(i + 1);
+    use(i, f);
+    WHA_FENCE();
+    f = next;
+  }
+}
+template <class F, int N>
+struct Frags {
+  F f[N];
+};
+
 // Whether a tile holds an infinity or NaN (one wave looks at all of it).
 template <class T, int DP, int ROWS>
 __device__ __forceinline__ bool tile_not_finite(const char* t, int lane) {
@@ -134,46 +153,67 @@ __device__ __forceinline__ bool tile_not_finite(const char* t, int lane) {
   return __builtin_amdgcn_ballot_w64(bad) != 0;
 }
 
-// acc[d][column] += sum over the tile's rows that belong to the column of
-// p[row][column] x[row][d].  As an MFMA wherever a weight of zero times x is
-// zero; where the mask cuts through the tile and x holds an infinity or NaN (0 x
-// inf), row by row over the rows the mask leaves.
-template <class T, int DP, int NDT, int NSUB, class Mine>
-__device__ __forceinline__ void add_rows(const char* t, const floatx16 (&p)[NSUB], floatx16 (&acc)[NDT], int lane,
-                                         Mine&& mine) {
-  const int g = lane >> 5, c = lane & 31;
-#pragma unroll 1
-  for (int x = 0; x < 32 * NSUB; ++x) {
-    const int i = 4 * ((x & 31) >> 3) + (x & 3), h = (x >> 2) & 1;
-    float px = 0.f;
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) px = s == (x >> 5) && j == i ? p[s][j] : px;
-    px = __shfl(px, c + 32 * h, 64);
-    if (mine(x)) {
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int y = 0; y < 16; ++y)
-          acc[dt][y] = fmaf(px, LdsTile<T, DP>::one(t, x, 32 * dt + row32(y, g)), acc[dt][y]);
-    }
-  }
-}
+// acc[d][column] += sum over the tile's rows of p[row][column] x[row][d]; weights of
+// rows that do not belong to a column are zero.
 template <class T, int DP, int NDT, int NSUB>
 __device__ __forceinline__ void add_cols(const char* t, const floatx16 (&p)[NSUB], floatx16 (&acc)[NDT], int lane) {
+  typename Elem<T>::Frag f[2 * NSUB];
 #pragma unroll
-  for (int s = 0; s < NSUB; ++s)
+  for (int s = 0; s < 2 * NSUB; ++s) {
+    float x[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float x[8];
+    for (int j = 0; j < 8; ++j) x[j] = p[s / 2][8 * (s & 1) + j];
+    f[s] = Elem<T>::pack(x);
+  }
+  one_ahead<2 * NSUB * NDT>([&](int i) { return LdsTile<T, DP>::cols32(t, i / NDT, i % NDT, lane); },
+                            [&](int i, const typename Elem<T>::Frag& x) {
+                              acc[i % NDT] = Elem<T>::mma32(x, f[i / NDT], acc[i % NDT]);
+                            });
+}
+
+// A weight of zero does not undo an infinity or NaN (0 x inf).  So where the mask
+// cuts through a tile that holds one, a wave leaves that tile's products and those
+// of the cut tiles after it out of its loop, and forms them here at the end: the
+// scores once more from memory, then row by row over the rows the mask leaves.  At
+// the end, because a second form of the products inside the loop costs the whole
+// kernel 60 registers and more.
+//
+// x y^T of 32 rows of memory each, by lane % 32.
+template <class T, int NKS, bool VEC>
+__device__ __forceinline__ floatx16 scores_of(const T* x, const T* y, int g, int D) {
+  floatx16 s = zeros16();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = p[s][8 * h + j];
-      const typename Elem<T>::Frag f = Elem<T>::pack(x);
+  for (int ks = 0; ks < NKS; ++ks) {
+    s = Elem<T>::mma32(row_frag<T, VEC>(x, ks, g, D), row_frag<T, VEC>(y, ks, g, D), s);
+    WHA_FENCE();
+  }
+  return s;
+}
+// acc[d][column] += p[row][column] row(x)[d] over the rows x with mine(x), of 32, the
+// weights by way of `w` (32 x 32 of the wave's own LDS).
+template <class T, int NDT, class Row, class Mine>
+__device__ __forceinline__ void add_rows(const floatx16& p, floatx16 (&acc)[NDT], T* w, int lane, int D, Row&& row,
+                                         Mine&& mine) {
+  const int g = lane >> 5, c = lane & 31;
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-        acc[dt] = Elem<T>::mma32(LdsTile<T, DP>::cols32(t, 2 * s + h, dt, lane), f, acc[dt]);
-    }
+  for (int i = 0; i < 16; ++i) w[row32(i, g) * 32 + c] = (T)p[i];
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+  for (int x = 0; x < 32; ++x) {
+    if (!mine(x)) continue;
+    const float px = (float)w[x * 32 + c];
+    const T* src = row(x);
+    int dim = D;
+    pin(dim);  // or 64 lane masks are held in registers
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const int d = 32 * dt + row32(y, g);
+        if (d < dim) acc[dt][y] = fmaf(px, (float)src[d], acc[dt][y]);
+      }
+  }
+  __builtin_amdgcn_wave_barrier();
 }
 
 }  // namespace
@@ -218,16 +258,18 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) o[dt] = zeros16();
 
+  int left = n_w;  // the first cut tile left to the end
   auto tile = [&](int kt, const char* Kt, const char* Vt) {
     const int k0 = kt * KT;
+    int ln = lane;
+    pin(ln);
     floatx16 s[NSUB];
 #pragma unroll
-    for (int x = 0; x < NSUB; ++x) {
-      s[x] = zeros16();
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks)
-        s[x] = Elem<T>::mma32(L::rows32(Kt, 32 * x + (lane & 31), ks, g), qf[ks], s[x]);
-    }
+    for (int x = 0; x < NSUB; ++x) s[x] = zeros16();
+    one_ahead<NSUB * NKS>([&](int i) { return L::rows32(Kt, 32 * (i / NKS), i % NKS, ln); },
+                          [&](int i, const typename Elem<T>::Frag& f) {
+                            s[i / NKS] = Elem<T>::mma32(f, qf[i % NKS], s[i / NKS]);
+                          });
     const bool cut = k0 + KT - 1 > t_first;  // wave-uniform: the mask cuts through the tile
     if (cut) {
 #pragma unroll
@@ -261,10 +303,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
         s[x][i] = fast_exp2(fmaf(s[x][i], sl2, -sub));
         l += s[x][i];
       }
-    if (cut && tile_not_finite<T, DP, KT>(Vt, lane))
-      add_rows<T, DP>(Vt, s, o, lane, [&](int x) { return k0 + x <= t; });
-    else
-      add_cols<T, DP>(Vt, s, o, lane);
+    if (cut && kt < left && tile_not_finite<T, DP, KT>(Vt, lane)) left = kt;
+    if (kt < left) add_cols<T, DP>(Vt, s, o, ln);
   };
   auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
     if constexpr (VEC) wait_vmem();
@@ -276,6 +316,18 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
     step(kt, K0, V0, K1, V1);
     if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
   }
+  __syncthreads();  // the tiles' LDS is free
+  if (left < n_w) {
+    T* w = reinterpret_cast<T*>(K0) + wave * 1024;
+    for (int k0 = left * KT; k0 < n_w * KT; k0 += 32) {
+      floatx16 s = scores_of<T, NKS, VEC>(Kb + (int64_t)min(k0 + (lane & 31), pl.len - 1) * a.k_st, Qr, g, D);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], sl2, -(m == -INFINITY ? 0.f : m)));
+      add_rows<T>(
+          s, o, w, lane, D, [&](int x) { return Vb + (int64_t)min(k0 + x, pl.len - 1) * a.v_st; },
+          [&](int x) { return k0 + x <= t; });
+    }
+  }
   l = pair_sum32(l);
   if (r < rows) {
     store_row<T, NDT, VEC>(O + (int64_t)(pl.start + t) * a.o_st + (int64_t)h * a.o_sh, D, g, o, 1.f / l);
@@ -284,10 +336,14 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
 }
 
 // ---------------------------------------------------------------- backward
+// (fp32 rows of 128 fill a wave's registers with two operands and a result: one
+// wave to a SIMD, without spills)
+constexpr int waves_per_simd(int size, int ndt) { return size == 4 && ndt > 2 ? 1 : 2; }
+
 // Query-stationary: dQ, and the row statistics lse log2(e) and Delta that the
 // key-stationary kernel reads.
 template <class T, int NKS, int NDT, bool VEC>
-__global__ __launch_bounds__(256, 2) void packed_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+__global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                            const T* __restrict__ V, const T* __restrict__ O,
                                                            const T* __restrict__ DO, const float* __restrict__ LSE,
                                                            T* __restrict__ DQ, float* __restrict__ LSE2,
@@ -339,18 +395,25 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const T* __restrict__
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = zeros16();
 
+  int left = n_w;
   auto tile = [&](int kt, const char* Kt, const char* Vt) {
     const int k0 = kt * KT;
+    int ln = lane;
+    pin(ln);
     floatx16 ds[NSUB];
     const bool cut = k0 + KT - 1 > t_first;
 #pragma unroll
     for (int x = 0; x < NSUB; ++x) {
       floatx16 s = zeros16(), dp = zeros16();
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) {
-        s = Elem<T>::mma32(L::rows32(Kt, 32 * x + (lane & 31), ks, g), qf[ks], s);
-        dp = Elem<T>::mma32(L::rows32(Vt, 32 * x + (lane & 31), ks, g), dof[ks], dp);
-      }
+      typedef Frags<typename Elem<T>::Frag, 2> F2;
+      one_ahead<NKS>(
+          [&](int ks) {
+            return F2{{L::rows32(Kt, 32 * x, ks, ln), L::rows32(Vt, 32 * x, ks, ln)}};
+          },
+          [&](int ks, const F2& f) {
+            s = Elem<T>::mma32(f.f[0], qf[ks], s);
+            dp = Elem<T>::mma32(f.f[1], dof[ks], dp);
+          });
 #pragma unroll
       for (int i = 0; i < 16; ++i) ds[x][i] = fast_exp2(fmaf(s[i], sl2, -lse2)) * (dp[i] - delta);
       if (cut) {
@@ -358,10 +421,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const T* __restrict__
         for (int i = 0; i < 16; ++i) ds[x][i] = k0 + 32 * x + row32(i, g) > t ? 0.f : ds[x][i];
       }
     }
-    if (cut && tile_not_finite<T, DP, KT>(Kt, lane))
-      add_rows<T, DP>(Kt, ds, dq, lane, [&](int x) { return k0 + x <= t; });
-    else
-      add_cols<T, DP>(Kt, ds, dq, lane);
+    if (cut && kt < left && tile_not_finite<T, DP, KT>(Kt, lane)) left = kt;
+    if (kt < left) add_cols<T, DP>(Kt, ds, dq, ln);
   };
   auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
     if constexpr (VEC) wait_vmem();
@@ -373,6 +434,20 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const T* __restrict__
     step(kt, K0, V0, K1, V1);
     if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
   }
+  __syncthreads();
+  if (left < n_w) {
+    T* w = reinterpret_cast<T*>(K0) + wave * 1024;
+    for (int k0 = left * KT; k0 < n_w * KT; k0 += 32) {
+      const int64_t key = min(k0 + (lane & 31), pl.len - 1);
+      floatx16 s = scores_of<T, NKS, VEC>(Kb + key * a.k_st, Qr, g, D);
+      const floatx16 dp = scores_of<T, NKS, VEC>(Vb + key * a.v_st, DO + o_at, g, D);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], sl2, -lse2)) * (dp[i] - delta);
+      add_rows<T>(
+          s, dq, w, lane, D, [&](int x) { return Kb + (int64_t)min(k0 + x, pl.len - 1) * a.k_st; },
+          [&](int x) { return k0 + x <= t; });
+    }
+  }
   if (r < rows)
     store_row<T, NDT, VEC>(DQ + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh, D, g, dq, scale);
 }
@@ -380,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const T* __restrict__
 // Key-stationary: dK and dV of 128 keys, over the rows of the group that come
 // after them.
 template <class T, int NKS, int NDT, bool VEC>
-__global__ __launch_bounds__(256, 2) void packed_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
+__global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
                                                             const T* __restrict__ V, const T* __restrict__ DO,
                                                             const float* __restrict__ LSE2,
                                                             const float* __restrict__ DELTA, T* __restrict__ DK,
@@ -390,6 +465,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(const T* __restrict_
   constexpr int BYTES = QT * L::kRow;
   __shared__ __align__(16) char Q0[BYTES], Q1[BYTES], D0[BYTES], D1[BYTES];
   __shared__ __align__(16) float S0[64], S1[64];  // a tile's lse log2(e), then its Delta
+  __shared__ __align__(16) char VS[BN * L::kRow];  // V of the block's keys: in registers it would not fit beside K, dK, dV
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -434,29 +510,33 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(const T* __restrict_
   const int rt_w = key0 < pl.len ? key0 * G / QT : n_rt;  // the first tile with a row after some key of the wave
   stage_q(rt0, Q0, D0, S0);
 
-  typename Elem<T>::Frag kf[NKS], vf[NKS];
+  typename Elem<T>::Frag kf[NKS];
   const T* Kr = K + (int64_t)(pl.start + kc) * a.k_st + (int64_t)hk * a.k_sh;
-  const T* Vr = V + (int64_t)(pl.start + kc) * a.v_st + (int64_t)hk * a.v_sh;
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) {
-    kf[ks] = row_frag<T, VEC>(Kr, ks, g, D);
-    vf[ks] = row_frag<T, VEC>(Vr, ks, g, D);
-  }
+  for (int ks = 0; ks < NKS; ++ks) kf[ks] = row_frag<T, VEC>(Kr, ks, g, D);
+  stage<T, DP, BN, NT, VEC>(VS, D, tid, [&](int rr) {
+    return V + (int64_t)(pl.start + min(pl.tile * BN + rr, pl.len - 1)) * a.v_st + (int64_t)hk * a.v_sh;
+  });
+  const char* Vw = VS + wave * 32 * L::kRow;
   floatx16 dk[NDT], dv[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dk[dt] = zeros16(), dv[dt] = zeros16();
 
+  int left = n_rt;  // the first cut tile left to the end
+  // the mask (or the sequence's end) cuts through the tile
+  auto is_cut = [&](int rt) { return rt * QT < (key0 + 31) * G || rt * QT + QT > rows; };
   auto tile = [&](int rt, const char* Qt, const char* Dt, const float* St) {
     const int r0 = rt * QT;
+    int ln = lane;
+    pin(ln);
     floatx16 p[1], ds[1];
     floatx16 s = zeros16(), dp = zeros16();
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      s = Elem<T>::mma32(L::rows32(Qt, lane & 31, ks, g), kf[ks], s);
-      dp = Elem<T>::mma32(L::rows32(Dt, lane & 31, ks, g), vf[ks], dp);
-    }
-    // the mask (or the sequence's end) cuts through the tile
-    const bool cut = r0 < (key0 + 31) * G || r0 + QT > rows;
+    one_ahead<NKS>([&](int ks) { return L::rows32(Qt, 0, ks, ln); },
+                   [&](int ks, const typename Elem<T>::Frag& f) { s = Elem<T>::mma32(f, kf[ks], s); });
+    typedef Frags<typename Elem<T>::Frag, 2> F2;
+    one_ahead<NKS>([&](int ks) { return F2{{L::rows32(Dt, 0, ks, ln), L::rows32(Vw, 0, ks, ln)}}; },
+                   [&](int ks, const F2& f) { dp = Elem<T>::mma32(f.f[0], f.f[1], dp); });
+    const bool cut = is_cut(rt);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const floatx4 lse2 = *reinterpret_cast<const floatx4*>(St + 8 * u + 4 * g);
@@ -477,12 +557,10 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(const T* __restrict_
         ds[0][i] = in ? ds[0][i] : 0.f;
       }
     }
-    if (cut && (tile_not_finite<T, DP, QT>(Qt, lane) || tile_not_finite<T, DP, QT>(Dt, lane))) {
-      add_rows<T, DP>(Dt, p, dv, lane, mine);
-      add_rows<T, DP>(Qt, ds, dk, lane, mine);
-    } else {
-      add_cols<T, DP>(Dt, p, dv, lane);
-      add_cols<T, DP>(Qt, ds, dk, lane);
+    if (cut && rt < left && (tile_not_finite<T, DP, QT>(Qt, lane) || tile_not_finite<T, DP, QT>(Dt, lane))) left = rt;
+    if (!cut || rt < left) {
+      add_cols<T, DP>(Dt, p, dv, ln);
+      add_cols<T, DP>(Qt, ds, dk, ln);
     }
   };
   auto step = [&](int rt, char* Qt, char* Dt, float* St, char* Qn, char* Dn, float* Sn) {
@@ -494,6 +572,35 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(const T* __restrict_
   for (int rt = rt0; rt < n_rt; rt += 2) {
     step(rt, Q0, D0, S0, Q1, D1, S1);
     if (rt + 1 < n_rt) step(rt + 1, Q1, D1, S1, Q0, D0, S0);
+  }
+  __syncthreads();
+  if (left < n_rt) {
+    T* w = reinterpret_cast<T*>(Q0) + wave * 1024;
+    const T* Vr = V + (int64_t)(pl.start + kc) * a.v_st + (int64_t)hk * a.v_sh;
+    for (int rt = left; rt < n_rt; ++rt) {
+      if (!is_cut(rt)) continue;
+      const int r0 = rt * QT;
+      auto q_row = [&](int x) {
+        const int r = min(r0 + x, rows - 1);
+        return Qb + (int64_t)(r / G) * a.q_st + (int64_t)(r % G) * a.q_sh;
+      };
+      auto do_row = [&](int x) {
+        const int r = min(r0 + x, rows - 1);
+        return Db + (int64_t)(r / G) * a.o_st + (int64_t)(r % G) * a.o_sh;
+      };
+      auto mine = [&](int x) { return r0 + x >= first && r0 + x < rows; };
+      floatx16 p = scores_of<T, NKS, VEC>(q_row(lane & 31), Kr, g, D);
+      floatx16 ds = scores_of<T, NKS, VEC>(do_row(lane & 31), Vr, g, D);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = min(r0 + row32(i, g), rows - 1);
+        const int64_t at = stat0 + (int64_t)(r % G) * a.total + r / G;
+        p[i] = fast_exp2(fmaf(p[i], sl2, -LSE2[at]));
+        ds[i] = p[i] * (ds[i] - DELTA[at]);
+      }
+      add_rows<T>(p, dv, w, lane, D, do_row, mine);
+      add_rows<T>(ds, dk, w, lane, D, q_row, mine);
+    }
   }
   if (key < pl.len) {
     store_row<T, NDT, VEC>(DK + (int64_t)(pl.start + key) * a.k_st + (int64_t)hk * a.k_sh, D, g, dk, scale);

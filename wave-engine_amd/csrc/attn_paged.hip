@@ -430,27 +430,59 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const T* __restrict__
   }
 }
 
-// Joins the splits of one (sequence, query head).
+// Joins the splits of one (sequence, query head): the statistics by a wave, a
+// split a lane; the outputs with kJoin splits in flight.
+constexpr int kJoin = 8;
 template <class T>
-__global__ __launch_bounds__(128) void paged_join_kernel(const float* __restrict__ WS, T* __restrict__ O,
+__global__ __launch_bounds__(256) void paged_join_kernel(const float* __restrict__ WS, T* __restrict__ O,
                                                          float* __restrict__ LSE, PagedDecode a, int D, int shift,
                                                          int splits) {
-  const int b = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head, d = threadIdx.x;
+  __shared__ float weight[256], part[2 * 128];
+  const int b = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head, tid = threadIdx.x, lane = tid & 63;
   const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages << shift);
   const int per = split_tiles(len, splits), n = len > 0 ? ((len + kTile - 1) / kTile + per - 1) / per : 0;
   const float* src = WS + (int64_t)blockIdx.x * splits * (D + 2);
-  float top = -INFINITY;
-  for (int s = 0; s < n; ++s) top = vmax2(top, src[s * (D + 2)]);
-  const float sub = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, x = 0.f;
-  for (int s = 0; s < n; ++s) {
-    const float* p = src + s * (D + 2);
-    const float e = fast_exp2(p[0] - sub);
-    sum = fmaf(p[1], e, sum);
-    if (d < D) x = fmaf(p[2 + d], e, x);
+  if (tid < 64) {
+    float m[4], l[4], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = lane + 64 * i;
+      m[i] = s < n ? src[s * (D + 2)] : -INFINITY;
+      l[i] = s < n ? src[s * (D + 2) + 1] : 0.f;
+      top = vmax2(top, m[i]);
+    }
+    top = max16(top);
+    top = pair_max32(pair_max16(top));
+    const float sub = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = fast_exp2(m[i] - sub);
+      sum = fmaf(l[i], m[i], sum);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) sum += xor_shfl(sum, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) weight[lane + 64 * i] = m[i] / sum;
+    if (lane == 0 && LSE != nullptr) LSE[blockIdx.x] = len > 0 ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
   }
-  if (d < D) O[(int64_t)b * a.o_sb + (int64_t)h * a.o_sh + d] = (T)(len > 0 ? x / sum : 0.f);
-  if (d == 0 && LSE != nullptr) LSE[blockIdx.x] = len > 0 ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
+  __syncthreads();
+  const int d = tid & 127, half = tid >> 7;
+  float x = 0.f;
+  if (d < D) {
+    for (int s = half; s < n; s += 2 * kJoin) {
+      float y[kJoin];
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i) y[i] = s + 2 * i < n ? src[(s + 2 * i) * (D + 2) + 2 + d] : 0.f;
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i)
+        if (s + 2 * i < n) x = fmaf(weight[s + 2 * i], y[i], x);
+    }
+  }
+  part[tid] = x;
+  __syncthreads();
+  if (half == 0 && d < D)
+    O[(int64_t)b * a.o_sb + (int64_t)h * a.o_sh + d] = (T)(len > 0 ? part[d] + part[128 + d] : 0.f);
 }
 
 // ---------------------------------------------------------------- launches
@@ -486,7 +518,7 @@ hipError_t decode_t(const void* q, void* o, float* lse, float* ws, const PagedDe
     if (e != hipSuccess || splits == 1) return e;
   }
   TimingScope ts("paged_join", stream);
-  hipLaunchKernelGGL((paged_join_kernel<T>), dim3((unsigned)d.n_seq * d.n_head), dim3(128), 0, stream, ws,
+  hipLaunchKernelGGL((paged_join_kernel<T>), dim3((unsigned)d.n_seq * d.n_head), dim3(256), 0, stream, ws,
                      static_cast<T*>(o), lse, d, c.D, c.shift, splits);
   return hipGetLastError();
 }

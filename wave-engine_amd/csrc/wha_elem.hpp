@@ -100,6 +100,14 @@ struct Elem<_Float16> {
   }
 };
 
+// Keeps what is formed from x where it stands in program order (an empty
+// statement that x passes through).  The addresses that a tile's reads are made
+// from are formed again for every tile, from a pinned lane: held in registers
+// over the loop they cost the 128-wide kernels more than a wave has.
+template <class T>
+__device__ __forceinline__ void pin(T& x) {
+  asm volatile("" : "+v"(x));
+}
 __device__ __forceinline__ floatx16 zeros16() {
   floatx16 z;
 #pragma unroll
@@ -148,12 +156,12 @@ struct LdsTile {
     else if constexpr (kQuads == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
     else return ((r & 3) << 2) | ((r >> 2) & 3);
   }
-  // byte offset of quad c of row r
-  __device__ __forceinline__ static int at(int r, int c) { return r * kRow + ((c ^ swz(r)) << 4); }
+  // byte offset of quad c of row r (rows 16 apart are 16 kRow apart)
+  __device__ __forceinline__ static int at(int r, int c) { return (r * kRow + (swz(r) << 4)) ^ (c << 4); }
 
-  // d = 16 ks + 8 g .. + 7 of row r
-  __device__ __forceinline__ static typename Elem<T>::Frag rows32(const char* t, int r, int ks, int g) {
-    return rows(t, r, 2 * ks + g);
+  // d = 16 ks + 8 (lane / 32) .. + 7 of row r0 + lane % 32, r0 a multiple of 16
+  __device__ __forceinline__ static typename Elem<T>::Frag rows32(const char* t, int r0, int ks, int lane) {
+    return rows(t + r0 * kRow, lane & 31, 2 * ks + (lane >> 5));
   }
   // elements 8 c .. 8 c + 7 of row r
   __device__ __forceinline__ static typename Elem<T>::Frag rows(const char* t, int r, int c) {
@@ -166,7 +174,7 @@ struct LdsTile {
     }
   }
   // four rows r .. r + 3 of column d0 + (lane & 15), 16-bit types; all 16 lanes
-  // of a group pass the same r and d0 (both multiples of 4 and 16)
+  // of a group pass the same r and d0 (multiples of 4 and 16)
   __device__ __forceinline__ static shortx4 tr4(const char* t, int r, int d0, int lane) {
     const int i = lane & 15, row = r + (i >> 2), d = d0 + 4 * (i & 3);
     const char* p = t + at(row, d >> 3) + 2 * (d & 7);
@@ -181,13 +189,13 @@ struct LdsTile {
       const int d = 32 * dt + (lane & 31);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int r = 16 * ks + row32(j, g);
-        f[j] = *reinterpret_cast<const float*>(t + at(r, d >> 2) + 4 * (d & 3));
+        f[j] = *reinterpret_cast<const float*>(t + 16 * ks * kRow + at(row32(j, g), d >> 2) + 4 * (d & 3));
       }
       return f;
     } else {
       const int d0 = 32 * dt + 16 * ((lane >> 4) & 1);
-      const shortx4 a = tr4(t, 16 * ks + 4 * g, d0, lane), b = tr4(t, 16 * ks + 8 + 4 * g, d0, lane);
+      const char* t0 = t + 16 * ks * kRow;
+      const shortx4 a = tr4(t0, 4 * g, d0, lane), b = tr4(t0, 8 + 4 * g, d0, lane);
       return __builtin_bit_cast(typename Elem<T>::Frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
@@ -205,7 +213,7 @@ struct LdsTile {
       }
       return f;
     } else {
-      const shortx4 a = tr4(t, 4 * g, 16 * dt, lane), b = tr4(t, 16 + 4 * g, 16 * dt, lane);
+      const shortx4 a = tr4(t, 4 * g, 16 * dt, lane), b = tr4(t + 16 * kRow, 4 * g, 16 * dt, lane);
       return __builtin_bit_cast(typename Elem<T>::Frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
