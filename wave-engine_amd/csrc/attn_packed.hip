@@ -27,15 +27,52 @@ namespace wha {
 
 namespace {
 
-// Which tile of which sequence a block takes.  Sequence i has the slots from
-// floor(rows before it / BM) + i on, which is at least as many as it has tiles;
-// the others stay empty.  So the grid needs the total only, and a block finds its
-// sequence by comparing against 64 starts at a time.
+// Which tile of which sequence block number `order` takes (of one key-value head's).
+// A tile's level is the number of tiles that it sweeps less one: those before it in
+// its sequence, or with KEYS (tiles of keys, swept by the rows after them) those
+// after it.  Up to 64 sequences: the highest level first, whatever the sequence, so
+// that the longest sweeps start first and the short ones fill in behind them.  More
+// sequences: sequence i has the slots from floor(rows before it / BM) + i on, which
+// is at least as many as it has tiles; that needs no sum over the sequences, and so
+// many balance by themselves.  Either way the grid needs only the total.
 struct Place {
-  int tile, start, len;  // tile < 0: an empty slot
+  int tile, start, len;  // tile < 0: none left
 };
 __device__ __forceinline__ int seq_start(const int* cu, int i, int total) { return min(max(cu[i], 0), total); }
-__device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total, int G, int BM, int slot, int lane) {
+template <bool KEYS>
+__device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total, int G, int BM, int slots, int order,
+                                            int lane) {
+  Place p;
+  if (n_seq <= 64) {
+    int start = 0, len = 0;
+    if (lane < n_seq) {
+      start = seq_start(cu, lane, total);
+      len = max(0, seq_start(cu, lane + 1, total) - start);
+    }
+    const int n = (int)(((int64_t)len * G + BM - 1) / BM);
+    int most = 0, step = 1;
+    for (int i = 0; i < n_seq; ++i) most = max(most, __builtin_amdgcn_readlane(n, i));
+    while (step * 63 < most) step *= 64;
+    // the level that `order` falls into: 64 levels at a time, narrowing down
+    int level = 0, above = 0;  // above: tiles of higher levels than it
+    for (; step > 0; step >>= 6) {
+      const int x = level + lane * step;
+      int count = 0;  // tiles of level x and higher
+      for (int i = 0; i < n_seq; ++i) count += max(0, __builtin_amdgcn_readlane(n, i) - x);
+      const int c = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(count > order)) - 1;
+      if (c < 0) return Place{-1, 0, 0};  // fewer tiles than this in all
+      level += c * step;
+      if (c < 63) above = __builtin_amdgcn_readlane(count, c + 1);
+    }
+    uint64_t has = __builtin_amdgcn_ballot_w64(n > level);
+    for (int i = above; i < order; ++i) has &= has - 1;
+    const int seq = has != 0 ? __builtin_ctzll(has) : 0;
+    p.start = __builtin_amdgcn_readlane(start, seq);
+    p.len = __builtin_amdgcn_readlane(len, seq);
+    p.tile = KEYS ? __builtin_amdgcn_readlane(n, seq) - 1 - level : level;
+    return p;
+  }
+  const int slot = KEYS ? order : slots - 1 - order;
   int lo = 0, n = n_seq;
   while (n > 1) {  // at most 6 rounds: n shrinks 64-fold
     const int step = (n + 63) / 64, i = lo + lane * step;
@@ -46,7 +83,6 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
     n = min(step, n - c * step);
   }
   lo = __builtin_amdgcn_readfirstlane(lo);
-  Place p;
   p.start = __builtin_amdgcn_readfirstlane(seq_start(cu, lo, total));
   p.len = __builtin_amdgcn_readfirstlane(max(0, seq_start(cu, lo + 1, total) - p.start));
   p.tile = slot - (int)((int64_t)p.start * G / BM) - lo;
@@ -54,31 +90,64 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
   return p;
 }
 
-// Rows of a tile into LDS, ROWS x DP by NT threads: row(rr) is the address of
-// tile row rr.  VEC: direct-to-LDS loads, complete after wait_vmem; quads past
-// the head dim come from 16 zero bytes.
-template <class T, int DP, int ROWS, int NT, bool VEC, class Row>
-__device__ __forceinline__ void stage(char* lds, int D, int tid, Row&& row) {
+// A tile of rows into LDS, ROWS x DP by NT threads.  VEC: direct-to-LDS buffer loads
+// from `base`, the address of the tile's first row, complete after wait_vmem: a
+// lane's offsets stay the same from tile to tile, and what moves is the descriptor,
+// in scalar registers.  Offsets past its range read as zeros: rows behind the last
+// one, and quads past the head dim.
+constexpr int kPast = (int)0x80000000;
+template <class T, int DP, int ROWS, int NT>
+struct Stage {
   using L = LdsTile<T, DP>;
-  constexpr int PER = ROWS * L::kQuads / NT, Q = Elem<T>::kQuad;
+  static constexpr int PER = ROWS * L::kQuads / NT, Q = Elem<T>::kQuad;
   static_assert(ROWS * L::kQuads % NT == 0, "whole rounds");
+  __device__ __forceinline__ static int row(int p, int tid) { return (p * NT + tid) / L::kQuads; }
+  __device__ __forceinline__ static int quad(int p, int tid) {
+    return ((p * NT + tid) % L::kQuads) ^ L::swz(row(p, tid));
+  }
+  // byte offset of quad c of a row `off` elements from the base
+  __device__ __forceinline__ static int at(int64_t off, int c, int D) {
+    return c * Q < D ? (int)((off + c * Q) * (int)sizeof(T)) : kPast;
+  }
+  __device__ __forceinline__ static void dma(__amdgpu_buffer_rsrc_t r, int off, char* lds, int p, int tid) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        r, (void __attribute__((address_space(3)))*)(lds + (p * NT + (tid & ~63)) * 16), 16, off, 0, 0, 0);
+  }
+  // one element at a time, from the row at `src`
+  __device__ __forceinline__ static void copy(const T* src, char* lds, int p, int tid, int D) {
+    const int c = quad(p, tid);
+    T x[Q];
 #pragma unroll
-  for (int p = 0; p < PER; ++p) {
-    const int idx = p * NT + tid, rr = idx / L::kQuads, c = (idx % L::kQuads) ^ L::swz(rr);
-    const T* src = row(rr) + c * Q;
+    for (int e = 0; e < Q; ++e) x[e] = c * Q + e < D ? src[c * Q + e] : (T)0.f;
+    uintx4 y;
+    __builtin_memcpy(&y, x, 16);
+    *reinterpret_cast<uintx4*>(lds + (p * NT + tid) * 16) = y;
+  }
+  // rows row0 .. of one head, st elements apart, n of them in all
+  struct Lanes {
+    int off[PER];
+  };
+  template <bool VEC>
+  __device__ __forceinline__ static void lanes(Lanes& l, int64_t st, int D, int tid) {
     if constexpr (VEC) {
-      const float* s = c * Q < D ? reinterpret_cast<const float*>(src) : g_zero_quad;
-      dma_quad(s, reinterpret_cast<float*>(lds + (p * NT + (tid & ~63)) * 16));
-    } else {
-      T x[Q];
 #pragma unroll
-      for (int e = 0; e < Q; ++e) x[e] = c * Q + e < D ? src[e] : (T)0.f;
-      uintx4 y;
-      __builtin_memcpy(&y, x, 16);
-      *reinterpret_cast<uintx4*>(lds + idx * 16) = y;
+      for (int p = 0; p < PER; ++p) l.off[p] = at(row(p, tid) * st, quad(p, tid), D);
     }
   }
-}
+  template <bool VEC>
+  __device__ __forceinline__ static void head(const Lanes& l, const T* base, int row0, int n, int64_t st, int D,
+                                              char* lds, int tid) {
+    if constexpr (VEC) {
+      const int64_t left = ((int64_t)(min(n - row0, ROWS) - 1) * st + D) * (int64_t)sizeof(T);
+      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(base + (int64_t)row0 * st, (uint32_t)left);
+#pragma unroll
+      for (int p = 0; p < PER; ++p) dma(r, l.off[p], lds, p, tid);
+    } else {
+#pragma unroll
+      for (int p = 0; p < PER; ++p) copy(base + (int64_t)min(row0 + row(p, tid), n - 1) * st, lds, p, tid, D);
+    }
+  }
+};
 
 // d = 16 ks + 8 g .. + 7 of one row as a fragment (zero past the head dim).
 template <class T, bool VEC>
@@ -146,11 +215,14 @@ struct Frags {
 // Whether a tile holds an infinity or NaN (one wave looks at all of it).
 template <class T, int DP, int ROWS>
 __device__ __forceinline__ bool tile_not_finite(const char* t, int lane) {
-  bool bad = false;
-#pragma unroll 4
-  for (int i = lane; i < ROWS * LdsTile<T, DP>::kQuads; i += 64)
-    bad |= quad_not_finite<T>(*reinterpret_cast<const uintx4*>(t + 16 * i));
-  return __builtin_amdgcn_ballot_w64(bad) != 0;
+  unsigned bad = 0;
+#pragma unroll 1
+  for (int i = lane; i < ROWS * LdsTile<T, DP>::kQuads; i += 64) {
+    const uintx4 q = *reinterpret_cast<const uintx4*>(t + 16 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bad |= not_finite_bits<T>(q[e]);
+  }
+  return __builtin_amdgcn_ballot_w64(bad != 0) != 0;
 }
 
 // acc[d][column] += sum over the tile's rows of p[row][column] x[row][d]; weights of
@@ -218,6 +290,23 @@ __device__ __forceinline__ void add_rows(const floatx16& p, floatx16 (&acc)[NDT]
 
 }  // namespace
 
+// Whether a result of any wave of the block is not finite (bad: of this lane).
+__device__ __forceinline__ bool any_bad(bool bad, int* flags, int wave, int lane) {
+  const uint64_t some = __builtin_amdgcn_ballot_w64(bad);
+  if (lane == 0) flags[wave] = some != 0;
+  __syncthreads();
+  return (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
+}
+template <int NDT>
+__device__ __forceinline__ bool not_finite(const floatx16 (&x)[NDT]) {
+  float chk = 0.f;  // NaN if any is not finite
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) chk = fmaf(x[dt][i], 0.f, chk);
+  return chk != 0.f;
+}
+
 // ---------------------------------------------------------------- forward
 template <class T, int NKS, int NDT, bool VEC>
 __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K,
@@ -225,23 +314,27 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
                                                             float* __restrict__ LSE, PackedArgs a, float sl2) {
   constexpr int DP = 32 * NDT, NT = 256, BM = 128, KT = sizeof(T) == 4 ? 32 : 64, NSUB = KT / 32;
   using L = LdsTile<T, DP>;
+  using St = Stage<T, DP, KT, NT>;
   constexpr int BYTES = KT * L::kRow;
   __shared__ __align__(16) char K0[BYTES], K1[BYTES], V0[BYTES], V1[BYTES];
+  __shared__ int flags[4];
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // a key-value head's blocks share an XCD's L2 where there are 8 of them; the
-  // later tiles of a sequence, which sweep more keys, first
-  const int hk = blockIdx.x % a.HK, slot = a.slots - 1 - (int)(blockIdx.x / a.HK);
-  const Place pl = find_place(a.cu, a.n_seq, a.total, G, BM, slot, lane);
+  // a key-value head's blocks share an XCD's L2 where there are 8 of them
+  const int hk = blockIdx.x % a.HK;
+  const Place pl = find_place<false>(a.cu, a.n_seq, a.total, G, BM, a.slots, (int)(blockIdx.x / a.HK), lane);
   if (pl.tile < 0) return;
   const int rows = pl.len * G, r0 = pl.tile * BM + wave * 32;
   const int r = r0 + (lane & 31), rc = min(r, rows - 1), t = rc / G, h = hk * G + rc % G;
   const T* Kb = K + (int64_t)pl.start * a.k_st + (int64_t)hk * a.k_sh;
   const T* Vb = V + (int64_t)pl.start * a.v_st + (int64_t)hk * a.v_sh;
+  typename St::Lanes kl, vl;
+  St::template lanes<VEC>(kl, a.k_st, D, tid);
+  St::template lanes<VEC>(vl, a.v_st, D, tid);
   auto stage_kv = [&](int kt, char* Kd, char* Vd) {
-    stage<T, DP, KT, NT, VEC>(Kd, D, tid, [&](int rr) { return Kb + (int64_t)min(kt * KT + rr, pl.len - 1) * a.k_st; });
-    stage<T, DP, KT, NT, VEC>(Vd, D, tid, [&](int rr) { return Vb + (int64_t)min(kt * KT + rr, pl.len - 1) * a.v_st; });
+    St::template head<VEC>(kl, Kb, kt * KT, pl.len, a.k_st, D, Kd, tid);
+    St::template head<VEC>(vl, Vb, kt * KT, pl.len, a.v_st, D, Vd, tid);
   };
   const int n_kt = min(pl.tile * BM + BM - 1, rows - 1) / G / KT + 1;  // tiles that the block sweeps
   const int t_first = __builtin_amdgcn_readfirstlane(t), t_last = __builtin_amdgcn_readlane(t, 31);
@@ -253,12 +346,10 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) qf[ks] = row_frag<T, VEC>(Qr, ks, g, D);
 
-  float m = -INFINITY, l = 0.f;  // running maximum (log2 units), this lane's part of the row sum
+  float m, l;  // running maximum (log2 units), this lane's part of the row sum
   floatx16 o[NDT];
-#pragma unroll
-  for (int dt = 0; dt < NDT; ++dt) o[dt] = zeros16();
-
-  int left = n_w;  // the first cut tile left to the end
+  bool check = false;
+  int left;  // the first cut tile left to the end
   auto tile = [&](int kt, const char* Kt, const char* Vt) {
     const int k0 = kt * KT;
     int ln = lane;
@@ -303,7 +394,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
         s[x][i] = fast_exp2(fmaf(s[x][i], sl2, -sub));
         l += s[x][i];
       }
-    if (cut && kt < left && tile_not_finite<T, DP, KT>(Vt, lane)) left = kt;
+    if (check && cut && kt < left && tile_not_finite<T, DP, KT>(Vt, lane)) left = kt;
     if (kt < left) add_cols<T, DP>(Vt, s, o, ln);
   };
   auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
@@ -312,13 +403,22 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
     if (kt + 1 < n_kt) stage_kv(kt + 1, Kn, Vn);
     if (kt < n_w) tile(kt, Kt, Vt);
   };
-  for (int kt = 0; kt < n_kt; kt += 2) {
-    step(kt, K0, V0, K1, V1);
-    if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
+  for (;;) {
+    m = -INFINITY, l = 0.f, left = n_w;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = zeros16();
+    for (int kt = 0; kt < n_kt; kt += 2) {
+      step(kt, K0, V0, K1, V1);
+      if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
+    }
+    // an infinity or NaN: once more, with an eye on the tiles that the mask cuts
+    if (check || !any_bad(r < rows && not_finite(o), flags, wave, lane)) break;
+    check = true;
+    stage_kv(0, K0, V0);
   }
-  __syncthreads();  // the tiles' LDS is free
-  if (left < n_w) {
-    T* w = reinterpret_cast<T*>(K0) + wave * 1024;
+  if (check) {
+    __syncthreads();  // the tiles' LDS is free
+    T* w = reinterpret_cast<T*>(wave & 2 ? K1 : K0) + (wave & 1) * 1024;
     for (int k0 = left * KT; k0 < n_w * KT; k0 += 32) {
       floatx16 s = scores_of<T, NKS, VEC>(Kb + (int64_t)min(k0 + (lane & 31), pl.len - 1) * a.k_st, Qr, g, D);
 #pragma unroll
@@ -343,29 +443,32 @@ constexpr int waves_per_simd(int size, int ndt) { return size == 4 && ndt > 2 ? 
 // Query-stationary: dQ, and the row statistics lse log2(e) and Delta that the
 // key-stationary kernel reads.
 template <class T, int NKS, int NDT, bool VEC>
-__global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq_kernel(const T* __restrict__ Q, const T* __restrict__ K,
-                                                           const T* __restrict__ V, const T* __restrict__ O,
-                                                           const T* __restrict__ DO, const float* __restrict__ LSE,
-                                                           T* __restrict__ DQ, float* __restrict__ LSE2,
-                                                           float* __restrict__ DELTA, PackedArgs a, float sl2,
-                                                           float scale) {
+__global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq_kernel(
+    const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ O,
+    const T* __restrict__ DO, const float* __restrict__ LSE, T* __restrict__ DQ, float* __restrict__ LSE2,
+    float* __restrict__ DELTA, PackedArgs a, float sl2, float scale) {
   constexpr int DP = 32 * NDT, NT = 256, BM = 128, KT = sizeof(T) == 4 ? 32 : 64, NSUB = KT / 32;
   using L = LdsTile<T, DP>;
+  using St = Stage<T, DP, KT, NT>;
   constexpr int BYTES = KT * L::kRow;
   __shared__ __align__(16) char K0[BYTES], K1[BYTES], V0[BYTES], V1[BYTES];
+  __shared__ int flags[4];
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hk = blockIdx.x % a.HK, slot = a.slots - 1 - (int)(blockIdx.x / a.HK);
-  const Place pl = find_place(a.cu, a.n_seq, a.total, G, BM, slot, lane);
+  const int hk = blockIdx.x % a.HK;
+  const Place pl = find_place<false>(a.cu, a.n_seq, a.total, G, BM, a.slots, (int)(blockIdx.x / a.HK), lane);
   if (pl.tile < 0) return;
   const int rows = pl.len * G, r0 = pl.tile * BM + wave * 32;
   const int r = r0 + (lane & 31), rc = min(r, rows - 1), t = rc / G, h = hk * G + rc % G;
   const T* Kb = K + (int64_t)pl.start * a.k_st + (int64_t)hk * a.k_sh;
   const T* Vb = V + (int64_t)pl.start * a.v_st + (int64_t)hk * a.v_sh;
+  typename St::Lanes kl, vl;
+  St::template lanes<VEC>(kl, a.k_st, D, tid);
+  St::template lanes<VEC>(vl, a.v_st, D, tid);
   auto stage_kv = [&](int kt, char* Kd, char* Vd) {
-    stage<T, DP, KT, NT, VEC>(Kd, D, tid, [&](int rr) { return Kb + (int64_t)min(kt * KT + rr, pl.len - 1) * a.k_st; });
-    stage<T, DP, KT, NT, VEC>(Vd, D, tid, [&](int rr) { return Vb + (int64_t)min(kt * KT + rr, pl.len - 1) * a.v_st; });
+    St::template head<VEC>(kl, Kb, kt * KT, pl.len, a.k_st, D, Kd, tid);
+    St::template head<VEC>(vl, Vb, kt * KT, pl.len, a.v_st, D, Vd, tid);
   };
   const int n_kt = min(pl.tile * BM + BM - 1, rows - 1) / G / KT + 1;
   const int t_first = __builtin_amdgcn_readfirstlane(t), t_last = __builtin_amdgcn_readlane(t, 31);
@@ -392,10 +495,8 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
     DELTA[stat_at] = delta;
   }
   floatx16 dq[NDT];
-#pragma unroll
-  for (int dt = 0; dt < NDT; ++dt) dq[dt] = zeros16();
-
-  int left = n_w;
+  bool check = false;
+  int left;
   auto tile = [&](int kt, const char* Kt, const char* Vt) {
     const int k0 = kt * KT;
     int ln = lane;
@@ -406,14 +507,11 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
     for (int x = 0; x < NSUB; ++x) {
       floatx16 s = zeros16(), dp = zeros16();
       typedef Frags<typename Elem<T>::Frag, 2> F2;
-      one_ahead<NKS>(
-          [&](int ks) {
-            return F2{{L::rows32(Kt, 32 * x, ks, ln), L::rows32(Vt, 32 * x, ks, ln)}};
-          },
-          [&](int ks, const F2& f) {
-            s = Elem<T>::mma32(f.f[0], qf[ks], s);
-            dp = Elem<T>::mma32(f.f[1], dof[ks], dp);
-          });
+      one_ahead<NKS>([&](int ks) { return F2{{L::rows32(Kt, 32 * x, ks, ln), L::rows32(Vt, 32 * x, ks, ln)}}; },
+                     [&](int ks, const F2& f) {
+                       s = Elem<T>::mma32(f.f[0], qf[ks], s);
+                       dp = Elem<T>::mma32(f.f[1], dof[ks], dp);
+                     });
 #pragma unroll
       for (int i = 0; i < 16; ++i) ds[x][i] = fast_exp2(fmaf(s[i], sl2, -lse2)) * (dp[i] - delta);
       if (cut) {
@@ -421,7 +519,7 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
         for (int i = 0; i < 16; ++i) ds[x][i] = k0 + 32 * x + row32(i, g) > t ? 0.f : ds[x][i];
       }
     }
-    if (cut && kt < left && tile_not_finite<T, DP, KT>(Kt, lane)) left = kt;
+    if (check && cut && kt < left && tile_not_finite<T, DP, KT>(Kt, lane)) left = kt;
     if (kt < left) add_cols<T, DP>(Kt, ds, dq, ln);
   };
   auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
@@ -430,13 +528,21 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
     if (kt + 1 < n_kt) stage_kv(kt + 1, Kn, Vn);
     if (kt < n_w) tile(kt, Kt, Vt);
   };
-  for (int kt = 0; kt < n_kt; kt += 2) {
-    step(kt, K0, V0, K1, V1);
-    if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
+  for (;;) {
+    left = n_w;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) dq[dt] = zeros16();
+    for (int kt = 0; kt < n_kt; kt += 2) {
+      step(kt, K0, V0, K1, V1);
+      if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
+    }
+    if (check || !any_bad(r < rows && not_finite(dq), flags, wave, lane)) break;
+    check = true;
+    stage_kv(0, K0, V0);
   }
-  __syncthreads();
-  if (left < n_w) {
-    T* w = reinterpret_cast<T*>(K0) + wave * 1024;
+  if (check) {
+    __syncthreads();
+    T* w = reinterpret_cast<T*>(wave & 2 ? K1 : K0) + (wave & 1) * 1024;
     for (int k0 = left * KT; k0 < n_w * KT; k0 += 32) {
       const int64_t key = min(k0 + (lane & 31), pl.len - 1);
       floatx16 s = scores_of<T, NKS, VEC>(Kb + key * a.k_st, Qr, g, D);
@@ -452,81 +558,91 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
     store_row<T, NDT, VEC>(DQ + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh, D, g, dq, scale);
 }
 
-// Key-stationary: dK and dV of 128 keys, over the rows of the group that come
-// after them.
-template <class T, int NKS, int NDT, bool VEC>
-__global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dkv_kernel(const T* __restrict__ Q, const T* __restrict__ K,
-                                                            const T* __restrict__ V, const T* __restrict__ DO,
-                                                            const float* __restrict__ LSE2,
-                                                            const float* __restrict__ DELTA, T* __restrict__ DK,
-                                                            T* __restrict__ DV, PackedArgs a, float sl2, float scale) {
-  constexpr int DP = 32 * NDT, NT = 256, BN = 128, QT = 32;
+// Key-stationary: dK and dV of 32 KG keys, over the rows of the group that come
+// after them: KG waves of 32 keys each, times 4 / KG that take every other 32 rows
+// and are added up at the end (KG = 2: where blocks of 128 keys are too few for the
+// CUs).
+template <class T, int NKS, int NDT, int KG, bool VEC>
+__global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dkv_kernel(
+    const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ DO,
+    const float* __restrict__ LSE2, const float* __restrict__ DELTA, T* __restrict__ DK, T* __restrict__ DV,
+    PackedArgs a, float sl2, float scale) {
+  static_assert(KG == 4 || KG == 2, "one or two row groups");
+  constexpr int DP = 32 * NDT, NT = 256, BN = 32 * KG, RG = 4 / KG, QT = 32 * RG;
   using L = LdsTile<T, DP>;
+  using St = Stage<T, DP, QT, NT>;
+  using StV = Stage<T, DP, BN, NT>;
   constexpr int BYTES = QT * L::kRow;
   __shared__ __align__(16) char Q0[BYTES], Q1[BYTES], D0[BYTES], D1[BYTES];
-  __shared__ __align__(16) float S0[64], S1[64];  // a tile's lse log2(e), then its Delta
+  __shared__ __align__(16) float S0[2 * QT], S1[2 * QT];  // a tile's lse log2(e), then its Delta
   __shared__ __align__(16) char VS[BN * L::kRow];  // V of the block's keys: in registers it would not fit beside K, dK, dV
+  __shared__ int flags[4];
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // the earlier keys of a sequence, which more rows come after, first
-  const int hk = blockIdx.x % a.HK, slot = (int)(blockIdx.x / a.HK);
-  const Place pl = find_place(a.cu, a.n_seq, a.total, 1, BN, slot, lane);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave % KG, rg = wave / KG;
+  const int hk = blockIdx.x % a.HK;
+  const Place pl = find_place<true>(a.cu, a.n_seq, a.total, 1, BN, a.slots, (int)(blockIdx.x / a.HK), lane);
   if (pl.tile < 0) return;
-  const int rows = pl.len * G, key0 = pl.tile * BN + wave * 32;
+  const int rows = pl.len * G, key0 = pl.tile * BN + kg * 32;
   const int key = key0 + (lane & 31), kc = min(key, pl.len - 1);
   const int first = key * G;  // the first row that comes at or after the key
   const T* Qb = Q + (int64_t)pl.start * a.q_st + (int64_t)hk * G * a.q_sh;
   const T* Db = DO + (int64_t)pl.start * a.o_st + (int64_t)hk * G * a.o_sh;
+  const T* Vb = V + (int64_t)pl.start * a.v_st + (int64_t)hk * a.v_sh;
   const int64_t stat0 = (int64_t)hk * G * a.total + pl.start;
-  // position and head of a tile's row (G <= 128: a 16-bit reciprocal is exact
-  // below 512)
+  // position and head of row rr of a tile (G <= 128: a 16-bit reciprocal is exact
+  // below 512); rows behind the last one repeat it
   const int magic = 65535 / G + 1;
   auto stage_q = [&](int rt, char* Qd, char* Dd, float* Sd) {
-    const int t0 = rt * QT / G, g0 = rt * QT % G;
+    const int t0 = rt * QT / G, g0 = rt * QT % G, end = rows - 1 - rt * QT;
     auto place = [&](int rr, int& t, int& gq) {
-      const int x = min(rr, rows - 1 - rt * QT) + g0, y = (x * magic) >> 16;
-      t = t0 + y;
-      gq = x - y * G;
+      const int x = min(rr, end) + g0;
+      t = (x * magic) >> 16;
+      gq = x - t * G;
     };
-    stage<T, DP, QT, NT, VEC>(Qd, D, tid, [&](int rr) {
+    const T *q = Qb + (int64_t)t0 * a.q_st, *d = Db + (int64_t)t0 * a.o_st;
+#pragma unroll
+    for (int p = 0; p < St::PER; ++p) {
       int t, gq;
-      place(rr, t, gq);
-      return Qb + (int64_t)t * a.q_st + (int64_t)gq * a.q_sh;
-    });
-    stage<T, DP, QT, NT, VEC>(Dd, D, tid, [&](int rr) {
+      place(St::row(p, tid), t, gq);
+      if constexpr (VEC) {
+        const int c = St::quad(p, tid);
+        St::dma(buffer_rsrc(q, 0x7fffffffu), St::at((int)(t * a.q_st + gq * a.q_sh), c, D), Qd, p, tid);
+        St::dma(buffer_rsrc(d, 0x7fffffffu), St::at((int)(t * a.o_st + gq * a.o_sh), c, D), Dd, p, tid);
+      } else {
+        St::copy(q + t * a.q_st + gq * a.q_sh, Qd, p, tid, D);
+        St::copy(d + t * a.o_st + gq * a.o_sh, Dd, p, tid, D);
+      }
+    }
+    if (wave < RG) {  // 64 of the 2 QT statistics to a wave
       int t, gq;
-      place(rr, t, gq);
-      return Db + (int64_t)t * a.o_st + (int64_t)gq * a.o_sh;
-    });
-    if (wave == 0) {
-      int t, gq;
-      place(lane & 31, t, gq);
-      const int64_t at = stat0 + (int64_t)gq * a.total + t;
-      dma_dword(lane < 32 ? LSE2 + at : DELTA + at, Sd);
+      place((wave * 64 + lane) % QT, t, gq);
+      const int64_t at = stat0 + (int64_t)gq * a.total + t0 + t;
+      dma_dword((wave * 64 + lane < QT ? LSE2 : DELTA) + at, Sd + wave * 64);
     }
   };
   const int rt0 = pl.tile * BN * G / QT, n_rt = (rows + QT - 1) / QT;
-  const int rt_w = key0 < pl.len ? key0 * G / QT : n_rt;  // the first tile with a row after some key of the wave
+  // sub-tiles of 32 rows: the first with a row after some key of the wave
+  const int sub0 = key0 < pl.len ? key0 * G / 32 : 0x7fffffff;
+  {
+    typename StV::Lanes vl;
+    StV::template lanes<VEC>(vl, a.v_st, D, tid);
+    StV::template head<VEC>(vl, Vb, pl.tile * BN, pl.len, a.v_st, D, VS, tid);
+  }
   stage_q(rt0, Q0, D0, S0);
+  const char* Vw = VS + kg * 32 * L::kRow;
 
   typename Elem<T>::Frag kf[NKS];
   const T* Kr = K + (int64_t)(pl.start + kc) * a.k_st + (int64_t)hk * a.k_sh;
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) kf[ks] = row_frag<T, VEC>(Kr, ks, g, D);
-  stage<T, DP, BN, NT, VEC>(VS, D, tid, [&](int rr) {
-    return V + (int64_t)(pl.start + min(pl.tile * BN + rr, pl.len - 1)) * a.v_st + (int64_t)hk * a.v_sh;
-  });
-  const char* Vw = VS + wave * 32 * L::kRow;
   floatx16 dk[NDT], dv[NDT];
-#pragma unroll
-  for (int dt = 0; dt < NDT; ++dt) dk[dt] = zeros16(), dv[dt] = zeros16();
-
-  int left = n_rt;  // the first cut tile left to the end
-  // the mask (or the sequence's end) cuts through the tile
-  auto is_cut = [&](int rt) { return rt * QT < (key0 + 31) * G || rt * QT + QT > rows; };
-  auto tile = [&](int rt, const char* Qt, const char* Dt, const float* St) {
-    const int r0 = rt * QT;
+  bool check = false;
+  int left;  // the first cut sub-tile left to the end
+  // the mask (or the sequence's end) cuts through sub-tile x
+  auto is_cut = [&](int x) { return x * 32 < (key0 + 31) * G || x * 32 + 32 > rows; };
+  auto tile = [&](int rt, const char* Qt, const char* Dt, const float* St_) {
+    const int x = rt * RG + rg, r0 = x * 32;
     int ln = lane;
     pin(ln);
     floatx16 p[1], ds[1];
@@ -536,11 +652,11 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
     typedef Frags<typename Elem<T>::Frag, 2> F2;
     one_ahead<NKS>([&](int ks) { return F2{{L::rows32(Dt, 0, ks, ln), L::rows32(Vw, 0, ks, ln)}}; },
                    [&](int ks, const F2& f) { dp = Elem<T>::mma32(f.f[0], f.f[1], dp); });
-    const bool cut = is_cut(rt);
+    const bool cut = is_cut(x);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const floatx4 lse2 = *reinterpret_cast<const floatx4*>(St + 8 * u + 4 * g);
-      const floatx4 delta = *reinterpret_cast<const floatx4*>(St + 32 + 8 * u + 4 * g);
+      const floatx4 lse2 = *reinterpret_cast<const floatx4*>(St_ + 8 * u + 4 * g);
+      const floatx4 delta = *reinterpret_cast<const floatx4*>(St_ + QT + 8 * u + 4 * g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * u + e;
@@ -548,47 +664,58 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
         ds[0][i] = p[0][i] * (dp[i] - delta[e]);
       }
     }
-    auto mine = [&](int x) { return r0 + x >= first && r0 + x < rows; };
     if (cut) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const bool in = mine(row32(i, g));
+        const int row = r0 + row32(i, g);
+        const bool in = row >= first && row < rows;
         p[0][i] = in ? p[0][i] : 0.f;
         ds[0][i] = in ? ds[0][i] : 0.f;
       }
     }
-    if (cut && rt < left && (tile_not_finite<T, DP, QT>(Qt, lane) || tile_not_finite<T, DP, QT>(Dt, lane))) left = rt;
-    if (!cut || rt < left) {
+    if (check && cut && x < left && (tile_not_finite<T, DP, 32>(Qt, lane) || tile_not_finite<T, DP, 32>(Dt, lane)))
+      left = x;
+    if (!cut || x < left) {
       add_cols<T, DP>(Dt, p, dv, ln);
       add_cols<T, DP>(Qt, ds, dk, ln);
     }
   };
-  auto step = [&](int rt, char* Qt, char* Dt, float* St, char* Qn, char* Dn, float* Sn) {
+  auto step = [&](int rt, char* Qt, char* Dt, float* St_, char* Qn, char* Dn, float* Sn) {
     wait_vmem();
     __syncthreads();
     if (rt + 1 < n_rt) stage_q(rt + 1, Qn, Dn, Sn);
-    if (rt >= rt_w) tile(rt, Qt, Dt, St);
+    const int x = rt * RG + rg;
+    if (x >= sub0 && x * 32 < rows)
+      tile(rt, Qt + rg * 32 * L::kRow, Dt + rg * 32 * L::kRow, St_ + rg * 32);
   };
-  for (int rt = rt0; rt < n_rt; rt += 2) {
-    step(rt, Q0, D0, S0, Q1, D1, S1);
-    if (rt + 1 < n_rt) step(rt + 1, Q1, D1, S1, Q0, D0, S0);
+  for (;;) {
+    left = 0x7fffffff;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) dk[dt] = zeros16(), dv[dt] = zeros16();
+    for (int rt = rt0; rt < n_rt; rt += 2) {
+      step(rt, Q0, D0, S0, Q1, D1, S1);
+      if (rt + 1 < n_rt) step(rt + 1, Q1, D1, S1, Q0, D0, S0);
+    }
+    if (check || !any_bad(key < pl.len && (not_finite(dk) || not_finite(dv)), flags, wave, lane)) break;
+    check = true;
+    stage_q(rt0, Q0, D0, S0);
   }
-  __syncthreads();
-  if (left < n_rt) {
-    T* w = reinterpret_cast<T*>(Q0) + wave * 1024;
-    const T* Vr = V + (int64_t)(pl.start + kc) * a.v_st + (int64_t)hk * a.v_sh;
-    for (int rt = left; rt < n_rt; ++rt) {
-      if (!is_cut(rt)) continue;
-      const int r0 = rt * QT;
-      auto q_row = [&](int x) {
-        const int r = min(r0 + x, rows - 1);
+  __syncthreads();  // the tiles' LDS is free
+  if (check && left != 0x7fffffff) {
+    T* w = reinterpret_cast<T*>(wave & 2 ? Q1 : Q0) + (wave & 1) * 1024;
+    const T* Vr = Vb + (int64_t)kc * a.v_st;
+    for (int x = left; x * 32 < rows; x += RG) {
+      if (!is_cut(x)) continue;
+      const int r0 = x * 32;
+      auto q_row = [&](int y) {
+        const int r = min(r0 + y, rows - 1);
         return Qb + (int64_t)(r / G) * a.q_st + (int64_t)(r % G) * a.q_sh;
       };
-      auto do_row = [&](int x) {
-        const int r = min(r0 + x, rows - 1);
+      auto do_row = [&](int y) {
+        const int r = min(r0 + y, rows - 1);
         return Db + (int64_t)(r / G) * a.o_st + (int64_t)(r % G) * a.o_sh;
       };
-      auto mine = [&](int x) { return r0 + x >= first && r0 + x < rows; };
+      auto mine = [&](int y) { return r0 + y >= first && r0 + y < rows; };
       floatx16 p = scores_of<T, NKS, VEC>(q_row(lane & 31), Kr, g, D);
       floatx16 ds = scores_of<T, NKS, VEC>(do_row(lane & 31), Vr, g, D);
 #pragma unroll
@@ -601,6 +728,30 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
       add_rows<T>(p, dv, w, lane, D, do_row, mine);
       add_rows<T>(ds, dk, w, lane, D, q_row, mine);
     }
+  }
+  if constexpr (RG == 2) {  // the second row group's sums by way of LDS: dK in Q0 or Q1, dV in D0 or D1
+    __syncthreads();
+    float* k_sum = reinterpret_cast<float*>(kg ? Q1 : Q0) + lane;
+    float* v_sum = reinterpret_cast<float*>(kg ? D1 : D0) + lane;
+    static_assert(BYTES >= NDT * 16 * 64 * 4, "a wave's sums in one buffer");
+    if (rg == 1) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          k_sum[(16 * dt + i) * 64] = dk[dt][i];
+          v_sum[(16 * dt + i) * 64] = dv[dt][i];
+        }
+    }
+    __syncthreads();
+    if (rg == 1) return;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        dk[dt][i] += k_sum[(16 * dt + i) * 64];
+        dv[dt][i] += v_sum[(16 * dt + i) * 64];
+      }
   }
   if (key < pl.len) {
     store_row<T, NDT, VEC>(DK + (int64_t)(pl.start + key) * a.k_st + (int64_t)hk * a.k_sh, D, g, dk, scale);
@@ -638,10 +789,21 @@ hipError_t bwd_t(const void* q, const void* k, const void* v, const void* o, con
     if (e != hipSuccess) return e;
   }
   TimingScope ts("packed_bwd_dkv", stream);
-  a.slots = packed_slots(a, 128, 1);
-  hipLaunchKernelGGL((packed_dkv_kernel<T, NKS, NDT, VEC>), dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream,
-                     static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                     static_cast<const T*>(d_o), lse2, delta, static_cast<T*>(dk), static_cast<T*>(dv), a, sl2, scale);
+  auto launch = [&](auto kernel, int keys) {
+    a.slots = packed_slots(a, keys, 1);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream, static_cast<const T*>(q),
+                       static_cast<const T*>(k), static_cast<const T*>(v), static_cast<const T*>(d_o), lse2, delta,
+                       static_cast<T*>(dk), static_cast<T*>(dv), a, sl2, scale);
+  };
+  // blocks of 64 keys where 128 would leave CUs without a second block (16-bit rows
+  // of up to 64), or without one (they fill a CU alone)
+  if constexpr (sizeof(T) * NDT <= 8) {
+    if ((int64_t)a.total * a.HK < (sizeof(T) * NDT <= 4 ? 512 : 128) * 128) {
+      launch(packed_dkv_kernel<T, NKS, NDT, 2, VEC>, 64);
+      return hipGetLastError();
+    }
+  }
+  launch(packed_dkv_kernel<T, NKS, NDT, 4, VEC>, 128);
   return hipGetLastError();
 }
 

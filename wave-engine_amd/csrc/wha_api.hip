@@ -1467,6 +1467,15 @@ bool rows_aligned(size_t size, std::initializer_list<const wha_layout*> views,
   return true;
 }
 
+// 32-bit byte offsets within 64 positions of these views, all heads included
+bool tile_offsets_fit(size_t size, std::initializer_list<const wha_layout*> views) {
+  for (const wha_layout* L : views)
+    if ((L->stride_t + L->stride_h) > ((int64_t)1 << 31) ||
+        (64 * L->stride_t + L->H * L->stride_h + L->D) * (int64_t)size >= (int64_t)1 << 31)
+      return false;
+  return true;
+}
+
 int check_packed(const char* fn, const int32_t* cu, int32_t n_seq, int32_t dtype, const wha_layout* q,
                  const wha_layout* k, const wha_layout* v, const wha_layout* o, float scale, wha::PackedArgs* a) {
   int rc;
@@ -1544,7 +1553,8 @@ int wha_packed_fwd(const void* q, const void* k, const void* v, void* o, float* 
   const int rc = check_packed(fn, cu_seqlens, n_seq, dtype, q_layout, k_layout, v_layout, o_layout, scale, &a);
   if (rc) return rc;
   if (!q || !k || !v || !o) return fail(WHA_ERR_INVALID, "%s: q, k, v and o must be non-NULL", fn);
-  const bool vec = rows_aligned(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout}, {q, k, v, o});
+  const bool vec = rows_aligned(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout}, {q, k, v, o}) &&
+                   tile_offsets_fit(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout});
   const hipError_t e =
       wha::launch_packed_fwd(dtype, q, k, v, o, lse, a, vec, scale, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "wha_packed_fwd launch");
@@ -1571,7 +1581,8 @@ int wha_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
   if (!q || !k || !v || !o || !d_o || !lse || !dq || !dk || !dv)
     return fail(WHA_ERR_INVALID, "%s: every tensor pointer must be non-NULL", fn);
   const bool vec = rows_aligned(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout},
-                                {q, k, v, o, d_o, dq, dk, dv});
+                                {q, k, v, o, d_o, dq, dk, dv}) &&
+                   tile_offsets_fit(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout});
   hipStream_t s = static_cast<hipStream_t>(stream);
   void* ws = nullptr;
   if ((rc = resolve_workspace(workspace, workspace_bytes, wha_packed_bwd_workspace_size(q_layout), s, fn, &ws)))

@@ -117,20 +117,17 @@ __device__ __forceinline__ floatx16 zeros16() {
 // Row within a 32 x 32 result of element i of lane group g.
 __device__ __forceinline__ int row32(int i, int g) { return 8 * (i >> 2) + 4 * g + (i & 3); }
 
-// Whether any of 16 bytes of T is an infinity or NaN.
+// A bit set where an element of a register is an infinity or NaN: an exponent of
+// all ones, plus one, carries into the sign's place (and no further).
 template <class T>
-__device__ __forceinline__ bool quad_not_finite(uintx4 q) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (std::is_same<T, float>::value) {
-      bad |= (q[i] & 0x7f800000u) == 0x7f800000u;
-    } else {
-      constexpr unsigned e = std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u;
-      bad |= (q[i] & e) == e || (q[i] & (e << 16)) == (e << 16);
-    }
-  }
-  return bad;
+__device__ __forceinline__ unsigned not_finite_bits(unsigned x) {
+  constexpr unsigned e = std::is_same<T, float>::value      ? 0x7f800000u
+                         : std::is_same<T, _Float16>::value ? 0x7c007c00u
+                                                            : 0x7f807f80u;
+  constexpr unsigned one = std::is_same<T, float>::value      ? 0x00800000u
+                           : std::is_same<T, _Float16>::value ? 0x04000400u
+                                                              : 0x00800080u;
+  return ((x & e) + one) & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
 }
 
 // A tile of rows of DP elements in LDS, read both as the rows operand of
