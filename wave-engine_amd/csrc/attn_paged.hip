@@ -65,6 +65,13 @@ __device__ __forceinline__ Raw<C> load8(const C* row, int d, int D, bool on) {
   }
   return r;
 }
+// 16 bytes through a buffer descriptor, past whose end is zero; not to be kept in
+// the caches (every row of a cache is read once by a decode: 110 -> 96 us at one
+// sequence of 131072 keys, 8 heads of 128 in bf16).
+constexpr int kPastEnd = (int)0x80000000, kOnce = 2;
+__device__ __forceinline__ uintx4 buffer_load16(__amdgpu_buffer_rsrc_t r, int off) {
+  return __builtin_bit_cast(uintx4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, kOnce));
+}
 // As numbers.
 template <class C>
 __device__ __forceinline__ void widen(const Raw<C>& r, float (&x)[8]) {
@@ -77,19 +84,30 @@ __device__ __forceinline__ void widen(const Raw<C>& r, float (&x)[8]) {
     for (int e = 0; e < 8; ++e) x[e] = (float)f[e];
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (float)((int)(r.a[e >> 2] << (24 - 8 * (e & 3))) >> 24);
+    for (int e = 0; e < 8; ++e) x[e] = (float)(((r.a[e >> 2] ^ 0x80808080u) >> (8 * (e & 3))) & 255u) - 128.f;
   }
+}
+// Four 8-bit steps as two pairs of fp16: 0x6400 + u is 1024 + u, exactly.
+__device__ __forceinline__ uintx2 steps_f16(unsigned w) {
+  const unsigned u = w ^ 0x80808080u;
+  const f16x2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+  const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
+  const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
+  return uintx2{__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi)};
 }
 // As a fragment of the type that the products are formed in (8-bit steps are
 // exact in all of them).
-template <class T, class C>
-__device__ __forceinline__ typename Elem<T>::Frag as_frag(const Raw<C>& r) {
-  if constexpr (std::is_same<T, C>::value && sizeof(T) == 2) {
-    return __builtin_bit_cast(typename Elem<T>::Frag, r.a);
+template <class X, class C>
+__device__ __forceinline__ typename Elem<X>::Frag as_frag(const Raw<C>& r) {
+  if constexpr (std::is_same<X, C>::value && sizeof(X) == 2) {
+    return __builtin_bit_cast(typename Elem<X>::Frag, r.a);
+  } else if constexpr (std::is_same<X, _Float16>::value && std::is_same<C, int8_t>::value) {
+    const uintx2 a = steps_f16(r.a[0]), b = steps_f16(r.a[1]);
+    return __builtin_bit_cast(typename Elem<X>::Frag, (uintx4{a[0], a[1], b[0], b[1]}));
   } else {
     float x[8];
     widen(r, x);
-    return Elem<T>::pack(x);
+    return Elem<X>::pack(x);
   }
 }
 template <class T, bool VEC>
@@ -234,19 +252,44 @@ size_t paged_decode_floats(int64_t n_seq, int n_head, int HK, int D, int64_t cap
   return n == 1 ? 0 : (size_t)n_seq * n_head * n * (D + 2);
 }
 
+// The type that a decode's products are formed in: the element type, but fp16 for
+// 8-bit caches of the 16-bit types.  The steps turn into fp16 two at a time (bf16
+// has no packed arithmetic), and weights keep 11 bits.
+template <class T, class C>
+using Product = typename std::conditional<std::is_same<C, int8_t>::value && sizeof(T) == 2, _Float16, T>::type;
+
+// How a tile's rows are reached.  kElements: element by element, any head dim and
+// alignment.  kPages: 16-byte loads, the page looked up row by row.  kOnePage: pages
+// of at least a tile, which so lies in one, a run of memory: buffer loads whose
+// offsets never change and whose descriptor (in scalar registers) ends at the last
+// key, so that what lies behind it reads as zeros.  (8-bit rows: 16 of them to a
+// load, so head dims that are multiples of 16; with 8, lines are fetched twice.)
+enum Reach { kElements, kPages, kOnePage };
+
 // One block: a split of one sequence's keys for up to 16 query heads of one
 // key-value head; its waves take 32-key tiles in turn, each with a softmax of its
 // own, joined at the end.  S^T = K Q^T on 16 x 16 results (keys on rows, heads on
 // columns), and P^T is the other operand of O^T += V^T P^T as it stands; V goes
-// through LDS, which gives it transposed.  A wave loads the next tile's rows into
-// registers before it works on the present one.
-template <class T, class C, int NKS, bool VEC>
-__global__ __launch_bounds__(256) void paged_decode_kernel(const T* __restrict__ Q, T* __restrict__ O,
+// through LDS, which gives it transposed.  A wave loads the next tile's V as soon as
+// this one's is in LDS and its K as soon as the scores are formed.
+template <class T, class C, int NKS, Reach REACH>
+__global__ __launch_bounds__(256, REACH == kOnePage && sizeof(Product<T, C>) == 2 ? 3 : 1) void paged_decode_kernel(const T* __restrict__ Q, T* __restrict__ O,
                                                            float* __restrict__ LSE, float* __restrict__ WS,
-                                                           PagedDecode a, PagedCache c, int splits, float sl2) {
-  constexpr int DP = 32 * NKS, NDT = 2 * NKS, UPR = DP / 8, PER = kTile * UPR / 64;  // units of 8 elements
-  constexpr bool Q8 = std::is_same<C, int8_t>::value, SCALED_V = Q8 && std::is_same<T, _Float16>::value;
-  using L = LdsTile<T, DP>;
+                                                           const int* __restrict__ TABLE, PagedDecode a, PagedCache c,
+                                                           int splits, float sl2) {
+  using X = Product<T, C>;
+  constexpr bool VEC = REACH != kElements, Q8 = std::is_same<C, int8_t>::value;
+  // fp16 weights of 8-bit values are kept relative to a power of two not below any
+  // scale so far, and queries of another type to one not below any of their
+  // elements, so that they stay in the range that fp16 holds to full precision
+  constexpr bool SCALED_V = Q8 && std::is_same<X, _Float16>::value, SCALED_Q = !std::is_same<T, X>::value;
+  constexpr int DP = 32 * NKS, NDT = 2 * NKS;
+  // a load takes U elements of a row: UPR to a row, PER to a lane and tile of V
+  constexpr int U = REACH == kOnePage && Q8 ? 16 : 8, UPR = DP / U, PER = kTile * UPR / 64;
+  constexpr int QUADS = U * (int)sizeof(C) / 16;  // kOnePage: 16-byte loads of a unit
+  // lane group g's 8 elements of k-step ks
+  auto dim = [&](int ks, int g) { return U == 16 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g; };
+  using L = LdsTile<X, DP>;
   constexpr int VB = kTile * L::kRow, JB = kHeads * DP * 4;
   __shared__ __align__(16) char lds[kWaves * (VB > JB ? VB : JB)];
   __shared__ __align__(16) float stat[kWaves][2 * kTile];
@@ -259,68 +302,148 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const T* __restrict__
   const int P = 1 << c.shift;
   const int64_t cap = (int64_t)a.max_pages << c.shift;
   const int len0 = a.lens[b], len = (int)min((int64_t)max(len0, 0), cap);
-  const int* table = a.table + (int64_t)b * a.table_stride;
+  const int* table = TABLE + (int64_t)b * a.table_stride;
   const int per = split_tiles(len, splits), t_end = min((split + 1) * per, (len + kTile - 1) / kTile);
   if (splits > 1 && split * per >= t_end) return;  // the join knows which splits there are
 
   const C* Kc = static_cast<const C*>(c.k);
   const C* Vc = static_cast<const C*>(c.v);
-  typename Elem<T>::Frag qf[NKS];
-  {
-    const T* row = Q + (int64_t)b * a.q_sb + (int64_t)(h0 + min(n16, nh - 1)) * a.q_sh;
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) qf[ks] = as_frag<T, T>(load8<T, VEC>(row, 32 * ks + 8 * g, D, n16 < nh));
-  }
-  // the page of key k0 + lane % 32 of a tile: -1 past the end, -2 outside the cache
-  auto page_of = [&](int tile) {
-    const int key = tile * kTile + (lane & 31);
-    if (tile >= t_end || key >= len) return -1;
-    const int pg = table[key >> c.shift];
-    return pg < 0 || pg >= c.n_pages ? -2 : pg;
+  // The table's entry for key k0 + lane % 32 (kOnePage: for the tile, a scalar load),
+  // looked at one tile later only (page_of): loads come back in order, and a wait
+  // for this one would be a wait for the tile loaded before it.
+  auto entry_of = [&](int tile) {
+    const int key = min(min(tile, t_end) * kTile + (REACH == kOnePage ? 0 : lane & 31), max(len - 1, 0));
+    return len > 0 ? table[key >> c.shift] : 0;
   };
-  auto row_of = [&](int pg, int key) { return (((int64_t)pg * c.HK + hk) << c.shift) + (key & (P - 1)); };
-  Raw<C> kr[2 * NKS], vr[PER];
+  // its page: -1 past the end, -2 outside the cache
+  auto page_of = [&](int tile, int entry) {
+    if (tile >= t_end || tile * kTile + (REACH == kOnePage ? 0 : lane & 31) >= len) return -1;
+    return entry < 0 || entry >= c.n_pages ? -2 : entry;
+  };
+  auto row_of = [&](int pg, int key) { return (((int64_t)max(pg, 0) * c.HK + hk) << c.shift) + (key & (P - 1)); };
+  typename std::conditional<REACH == kOnePage, uintx4, Raw<C>>::type kr[REACH == kOnePage ? 2 * NKS * 8 / U * QUADS : 2 * NKS],
+      vr[REACH == kOnePage ? PER * QUADS : PER];
   float ksc = 0.f, vsc = 0.f;
-  auto load = [&](int tile, int pg) {
+  int k_off[2], v_off[PER];  // kOnePage: byte offsets in a tile
+  if constexpr (REACH == kOnePage) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int p = __shfl(pg, 16 * x + n16, 64);
-      const C* row = Kc + row_of(max(p, 0), tile * kTile + 16 * x + n16) * D;
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) kr[x * NKS + ks] = load8<C, VEC>(row, 32 * ks + 8 * g, D, p >= 0);
-    }
+    for (int x = 0; x < 2; ++x) k_off[x] = ((16 * x + n16) * D + U * g) * (int)sizeof(C);
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int r = (u * 64 + lane) / UPR, p = __shfl(pg, r, 64);
-      vr[u] = load8<C, VEC>(Vc + row_of(max(p, 0), tile * kTile + r) * D, 8 * (lane % UPR), D, p >= 0);
+      const int r = (u * 64 + lane) / UPR, d = U * (lane % UPR);
+      v_off[u] = d < D ? (r * D + d) * (int)sizeof(C) : kPastEnd;
     }
-    if constexpr (Q8) {
-      const int64_t row = row_of(max(pg, 0), tile * kTile + (lane & 31));
-      ksc = pg >= 0 ? c.ks[row] : 0.f;
-      vsc = pg >= 0 ? c.vs[row] : 0.f;
+  }
+  // keys of the tile, none where there is no page
+  auto keys = [&](int tile, int pg) { return pg >= 0 ? (uint32_t)min(kTile, len - tile * kTile) : 0u; };
+  auto load_k = [&](int tile, int pg) {
+    if constexpr (REACH == kOnePage) {
+      const int64_t row = row_of(pg, tile * kTile);
+      const uint32_t n = keys(tile, pg);
+      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(Kc + row * D, n * (uint32_t)(D * sizeof(C)));
+      constexpr int PR = NKS * 8 / U;  // units of a row to a lane, 4 U elements apart
+#pragma unroll
+      for (int i = 0; i < 2 * PR; ++i)
+#pragma unroll
+        for (int e = 0; e < QUADS; ++e)
+          kr[i * QUADS + e] = buffer_load16(
+              r, 4 * U * (i % PR) + U * g < D ? k_off[i / PR] + 4 * U * (i % PR) * (int)sizeof(C) + 16 * e : kPastEnd);
+      if constexpr (Q8) ksc = buffer_load_float(buffer_rsrc(c.ks + row, n * 4u), lane * 4, 0);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int p = __shfl(pg, 16 * x + n16, 64);
+        const C* row = Kc + row_of(p, tile * kTile + 16 * x + n16) * D;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) kr[x * NKS + ks] = load8<C, VEC>(row, dim(ks, g), D, p >= 0);
+      }
+      if constexpr (Q8) ksc = pg >= 0 ? c.ks[row_of(pg, tile * kTile + (lane & 31))] : 0.f;
     }
   };
+  auto load_v = [&](int tile, int pg) {
+    if constexpr (REACH == kOnePage) {
+      const int64_t row = row_of(pg, tile * kTile);
+      const uint32_t n = keys(tile, pg);
+      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(Vc + row * D, n * (uint32_t)(D * sizeof(C)));
+#pragma unroll
+      for (int u = 0; u < PER; ++u)
+#pragma unroll
+        for (int e = 0; e < QUADS; ++e) vr[u * QUADS + e] = buffer_load16(r, v_off[u] + 16 * e);
+      if constexpr (Q8) vsc = buffer_load_float(buffer_rsrc(c.vs + row, n * 4u), lane * 4, 0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const int r = (u * 64 + lane) / UPR, p = __shfl(pg, r, 64);
+        vr[u] = load8<C, VEC>(Vc + row_of(p, tile * kTile + r) * D, 8 * (lane % UPR), D, p >= 0);
+      }
+      if constexpr (Q8) vsc = pg >= 0 ? c.vs[row_of(pg, tile * kTile + (lane & 31))] : 0.f;
+    }
+  };
+  // the i-th 8 elements of a lane's loads
+  auto eight = [&](const auto& x, int i) {
+    Raw<C> r;
+    if constexpr (REACH != kOnePage) {
+      r = x[i];
+    } else if constexpr (sizeof(C) == 4) {
+      r.a = __builtin_bit_cast(floatx4, x[2 * i]);
+      r.b = __builtin_bit_cast(floatx4, x[2 * i + 1]);
+    } else if constexpr (sizeof(C) == 2) {
+      r.a = x[i];
+    } else {
+      r.a = (i & 1) ? uintx2{x[i / 2][2], x[i / 2][3]} : uintx2{x[i / 2][0], x[i / 2][1]};
+    }
+    return r;
+  };
+
+  int tile = split * per + wave, entry = entry_of(tile + kWaves), pg = page_of(tile, entry_of(tile));
+  load_v(tile, pg);
+  load_k(tile, pg);
+
+  typename Elem<X>::Frag qf[NKS];
+  {
+    const T* row = Q + (int64_t)b * a.q_sb + (int64_t)(h0 + min(n16, nh - 1)) * a.q_sh;
+    float x[NKS][8], top = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const Raw<T> r = load8<T, VEC>(row, dim(ks, g), D, n16 < nh);
+      if constexpr (SCALED_Q) {
+        widen(r, x[ks]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[ks][e]));
+      } else {
+        qf[ks] = as_frag<X, T>(r);
+      }
+    }
+    if constexpr (SCALED_Q) {
+      top = pair_max32(pair_max16(top));
+      const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+      sl2 = __builtin_amdgcn_ldexpf(sl2, e);
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[ks][i] = __builtin_amdgcn_ldexpf(x[ks][i], -e);
+        qf[ks] = Elem<X>::pack(x[ks]);
+      }
+    }
+  }
 
   float m = -INFINITY, l = 0.f, vref = 0.f;
   floatx4 o[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) o[dt] = floatx4{0.f, 0.f, 0.f, 0.f};
   char* Vt = lds + wave * VB;
-  int tile = split * per + wave, pg = page_of(tile), pg_next = page_of(tile + kWaves);
-  load(tile, pg);
   for (; tile < t_end; tile += kWaves) {
-    typename Elem<T>::Frag kf[2 * NKS];
+    int ln = lane;
+    pin(ln);
 #pragma unroll
-    for (int i = 0; i < 2 * NKS; ++i) kf[i] = as_frag<T, C>(kr[i]);
-#pragma unroll
-    for (int u = 0; u < PER; ++u) L::put(Vt, (u * 64 + lane) / UPR, lane % UPR, as_frag<T, C>(vr[u]));
-    float w = 1.f;
+    for (int i = 0; i < PER * U / 8; ++i) {
+      const int u = i / (U / 8), half = i % (U / 8);
+      L::put(Vt, (u * 64 + ln) / UPR, (ln % UPR) * (U / 8) + half, as_frag<X, C>(eight(vr, i)));
+    }
     if constexpr (Q8) {
-      // fp16 weights: relative to a power of two not below any scale so far, so that
-      // they stay in the range that fp16 holds to full precision
-      w = vsc;
+      float w = vsc;
       if constexpr (SCALED_V) {
-        float top = max16(vsc);
+        float top = max16(lane < kTile ? vsc : 0.f);
         top = pair_max32(pair_max16(top));
         if (top > vref) {  // wave-uniform
           const float now = __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(top));
@@ -339,32 +462,45 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const T* __restrict__
     const uint64_t out = __builtin_amdgcn_ballot_w64(pg == -2);
     const int k0 = tile * kTile;
     __builtin_amdgcn_wave_barrier();
-    load(tile + kWaves, pg_next);
-    pg = pg_next;
-    pg_next = page_of(tile + 2 * kWaves);
+    pg = page_of(tile + kWaves, entry);
+    load_v(tile + kWaves, pg);
     floatx4 s[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       s[x] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) s[x] = Elem<T>::mma16(kf[x * NKS + ks], qf[ks], s[x]);
-      if constexpr (Q8) s[x] *= *reinterpret_cast<const floatx4*>(&stat[wave][16 * x + 4 * g]);
+      for (int ks = 0; ks < NKS; ++ks) s[x] = Elem<X>::mma16(as_frag<X, C>(eight(kr, x * NKS + ks)), qf[ks], s[x]);
+    }
+    entry = entry_of(tile + 2 * kWaves);
+    load_k(tile + kWaves, pg);
+    if constexpr (Q8) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[x][i] = k0 + 16 * x + 4 * g + i < len ? s[x][i] : -INFINITY;
+      for (int x = 0; x < 2; ++x) s[x] *= *reinterpret_cast<const floatx4*>(&stat[wave][16 * x + 4 * g]);
+    }
+    if (k0 + kTile > len) {  // wave-uniform
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[x][i] = k0 + 16 * x + 4 * g + i < len ? s[x][i] : -INFINITY;
     }
     if (out != 0) {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if ((out >> (16 * x + 4 * g + i)) & 1) s[x][i] = __uint_as_float(0x7fc00000u);
+          if (REACH == kOnePage || ((out >> (16 * x + 4 * g + i)) & 1)) s[x][i] = __uint_as_float(0x7fc00000u);
     }
     float mx = vmax3(vmax3(s[0][0], s[0][1], s[0][2]), s[0][3], s[1][0]);
     mx = vmax3(vmax3(mx, s[1][1], s[1][2]), s[1][3], s[1][3]);
-    mx = vmax2(m, pair_max32(pair_max16(mx)) * sl2);
-    const float sub = mx == -INFINITY ? 0.f : mx, alpha = fast_exp2(m - sub);
-    m = mx;
-    l *= alpha;
+    mx = pair_max32(pair_max16(mx)) * sl2;
+    if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {  // (as in the packed forward)
+      const float mn = vmax2(m, mx), alpha = mn == m ? 1.f : fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+    }
+    const float sub = m == -INFINITY ? 0.f : m;
     float p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -379,11 +515,11 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const T* __restrict__
         for (int i = 0; i < 4; ++i) p[4 * x + i] *= y[i];
       }
     }
-    const typename Elem<T>::Frag pf = Elem<T>::pack(p);
+    const typename Elem<X>::Frag pf = Elem<X>::pack(p);
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
-      o[dt] *= alpha;
-      o[dt] = Elem<T>::mma16(L::cols16(Vt, dt, lane), pf, o[dt]);
+      o[dt] = Elem<X>::mma16(L::cols16(Vt, dt, ln), pf, o[dt]);
+      if (dt % 4 == 3) WHA_FENCE();
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -504,15 +640,15 @@ hipError_t read_t(void* k, void* v, const PagedRows& r, const PagedCache& c, hip
                      static_cast<T*>(k), static_cast<T*>(v), r, c);
   return hipGetLastError();
 }
-template <class T, class C, int NKS, bool VEC>
+template <class T, class C, int NKS, Reach REACH>
 hipError_t decode_t(const void* q, void* o, float* lse, float* ws, const PagedDecode& d, const PagedCache& c,
                     float scale, hipStream_t stream) {
   const int splits = paged_splits(d.n_seq, d.n_head, c.HK, (int64_t)d.max_pages << c.shift);
   const int groups = (d.n_head / c.HK + kHeads - 1) / kHeads;
   {
     TimingScope ts("paged_decode", stream);
-    hipLaunchKernelGGL((paged_decode_kernel<T, C, NKS, VEC>), dim3((unsigned)d.n_seq * groups * splits * c.HK),
-                       dim3(256), 0, stream, static_cast<const T*>(q), static_cast<T*>(o), lse, ws, d, c, splits,
+    hipLaunchKernelGGL((paged_decode_kernel<T, C, NKS, REACH>), dim3((unsigned)d.n_seq * groups * splits * c.HK),
+                       dim3(256), 0, stream, static_cast<const T*>(q), static_cast<T*>(o), lse, ws, d.table, d, c, splits,
                        (float)((double)scale * 1.4426950408889634));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
@@ -525,11 +661,14 @@ hipError_t decode_t(const void* q, void* o, float* lse, float* ws, const PagedDe
 template <class T, class C>
 hipError_t decode_c(const void* q, void* o, float* lse, float* ws, const PagedDecode& d, const PagedCache& c, bool vec,
                     float scale, hipStream_t stream) {
-  if (c.D <= 64)
-    return vec ? decode_t<T, C, 2, true>(q, o, lse, ws, d, c, scale, stream)
-               : decode_t<T, C, 2, false>(q, o, lse, ws, d, c, scale, stream);
-  return vec ? decode_t<T, C, 4, true>(q, o, lse, ws, d, c, scale, stream)
-             : decode_t<T, C, 4, false>(q, o, lse, ws, d, c, scale, stream);
+  auto dims = [&](auto reach) {
+    constexpr Reach R = decltype(reach)::value;
+    return c.D <= 64 ? decode_t<T, C, 2, R>(q, o, lse, ws, d, c, scale, stream)
+                     : decode_t<T, C, 4, R>(q, o, lse, ws, d, c, scale, stream);
+  };
+  if (!vec) return dims(std::integral_constant<Reach, kElements>{});
+  return (1 << c.shift) >= kTile && c.D * sizeof(C) % 16 == 0 ? dims(std::integral_constant<Reach, kOnePage>{})
+                                 : dims(std::integral_constant<Reach, kPages>{});
 }
 
 }  // namespace
