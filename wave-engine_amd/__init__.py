@@ -24,6 +24,7 @@ The directory name contains a hyphen, so it is loaded by path (see
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 import subprocess
@@ -250,6 +251,7 @@ def _same_layout(L, *ts):
             raise ValueError(f"all tensors must share one layout: {L} vs {l2}")
 
 
+@functools.lru_cache(maxsize=None)
 def default_scale(D: int) -> float:
     """1/sqrt(head_dim) rounded to f32, as src/common/compute.rs:362 computes it."""
     return float(np.float32(1.0) / np.sqrt(np.float32(D)))
@@ -500,30 +502,48 @@ def _index_tensor(t, name, dtype, device, dim=1):
                          f"got {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
-def _on_device(t):
-    """Kernels are launched with the tensors' device current, whichever is."""
+def _call(fn, device, *args):
+    """A launching entry point with the device's current stream as its last
+    argument, and the device current while it launches, whichever is."""
     torch = _torch()
-    import contextlib
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    L = lib()
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            rc = getattr(L, fn)(*args, _raw_stream(device))
+    else:
+        rc = getattr(L, fn)(*args, _raw_stream(device))
+    if rc != WHA_OK:
+        raise WaveHipError(fn, rc, L.wha_last_error().decode())
 
 
-def _lse_out(lse, shape, device):
+def _raw_stream(device):
+    """The current stream's handle (without the Stream object, which costs as much
+    as half a launch, where torch has a way)."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw else torch.cuda.current_stream(device).cuda_stream
+
+
+def _address(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _lse_out(lse, shape, like):
     torch = _torch()
     if lse is None:
-        return torch.empty(shape, dtype=torch.float32, device=device)
-    if tuple(lse.shape) != shape or lse.dtype != torch.float32 or lse.device != device or not lse.is_contiguous():
-        raise ValueError(f"lse: expected a contiguous float32 {shape} tensor on {device}")
+        return like.new_empty(shape, dtype=torch.float32)
+    if tuple(lse.shape) != shape or lse.dtype != torch.float32 or lse.device != like.device or not lse.is_contiguous():
+        raise ValueError(f"lse: expected a contiguous float32 {shape} tensor on {like.device}")
     return lse
 
 
-def _workspace(workspace, need, device):
+def _workspace(workspace, need, like):
     """(tensor, bytes) of a call's workspace: the caller's, or one from torch's
     allocator (safe under stream capture, unlike the library's cached one)."""
-    torch = _torch()
     if workspace is None:
-        return (torch.empty(need, dtype=torch.uint8, device=device), need) if need else (None, 0)
-    if workspace.device != device or not workspace.is_contiguous():
-        raise ValueError(f"workspace: expected a contiguous tensor on {device}")
+        return (like.new_empty(need, dtype=_torch().uint8), need) if need else (None, 0)
+    if workspace.device != like.device or not workspace.is_contiguous():
+        raise ValueError(f"workspace: expected a contiguous tensor on {like.device}")
     return workspace, workspace.numel() * workspace.element_size()
 
 
@@ -543,21 +563,19 @@ def packed_fwd(q, k, v, cu_seqlens, scale=None, want_lse=True, out=None, lse=Non
     device.  Returns (o, lse) with lse [H][N], or o alone when want_lse=False.
     Rows behind the last sequence are left as they were (in a new o and lse:
     whatever the allocator gave)."""
-    torch = _torch()
     Lq, Lk, Lv, n_seq = _packed_views(q, k, v, cu_seqlens)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape:
         raise ValueError(f"out: expected shape {tuple(q.shape)}, got {tuple(out.shape)}")
     Lo = _heads_layout(out, "out", q)
     code = _dtype_code(q.dtype, "q")
-    lse = _lse_out(lse, (Lq.H, Lq.T), q.device) if want_lse else None
+    lse = _lse_out(lse, (Lq.H, Lq.T), q) if want_lse else None
     if q.numel() and n_seq > 0:
         s = default_scale(Lq.D) if scale is None else float(scale)
-        with _on_device(q):
-            _check("wha_packed_fwd", lib().wha_packed_fwd(
-                _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cu_seqlens), n_seq, code, ctypes.byref(Lq),
-                ctypes.byref(Lk), ctypes.byref(Lv), ctypes.byref(Lo), s, _stream_ptr(q)))
+        ref = ctypes.byref
+        _call("wha_packed_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _address(lse),
+              cu_seqlens.data_ptr(), n_seq, code, ref(Lq), ref(Lk), ref(Lv), ref(Lo), s)
     return (out, lse) if want_lse else out
 
 
@@ -566,31 +584,31 @@ def packed_bwd(q, k, v, o, do, lse, cu_seqlens, scale=None, workspace=None, dq=N
     dv), which have the strides of q, k and v (given ones too: slices of a fused
     gradient where q, k and v are slices); do has those of o.  float32 and
     bfloat16."""
-    torch = _torch()
     Lq, Lk, Lv, n_seq = _packed_views(q, k, v, cu_seqlens)
     Lo = _heads_layout(o, "o", q)
     grads = []
     for t, g, name in ((q, dq, "dq"), (k, dk, "dk"), (v, dv, "dv"), (o, do, "do")):
         if g is None:
-            g = torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
-        elif g.shape != t.shape or any(n > 1 and a != b for n, a, b in zip(t.shape, g.stride(), t.stride())):
+            g = _torch().empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
+        elif g.shape != t.shape or (g.stride() != t.stride() and
+                                    any(n > 1 and a != b for n, a, b in zip(t.shape, g.stride(), t.stride()))):
             raise ValueError(f"{name} must have the shape and strides of {name[1:]}: {tuple(t.shape)} {t.stride()}, "
                              f"got {tuple(g.shape)} {g.stride()}")
-        _heads_layout(g, name, q)
+        elif g.dtype != t.dtype or g.device != t.device:
+            raise TypeError(f"{name}: expected {t.dtype} on {t.device}, got {g.dtype} on {g.device}")
         grads.append(g)
     if o.shape != q.shape:
         raise ValueError(f"o: expected shape {tuple(q.shape)}, got {tuple(o.shape)}")
     code = _dtype_code(q.dtype, "q")
-    lse = _lse_out(lse, (Lq.H, Lq.T), q.device)
+    lse = _lse_out(lse, (Lq.H, Lq.T), q)
     dq, dk, dv, do = grads
     if q.numel() and n_seq > 0:
         s = default_scale(Lq.D) if scale is None else float(scale)
-        with _on_device(q):
-            ws, ws_bytes = _workspace(workspace, int(lib().wha_packed_bwd_workspace_size(ctypes.byref(Lq))), q.device)
-            _check("wha_packed_bwd", lib().wha_packed_bwd(
-                _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(do), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv),
-                _ptr(cu_seqlens), n_seq, code, _ptr(ws), ws_bytes, ctypes.byref(Lq), ctypes.byref(Lk),
-                ctypes.byref(Lv), ctypes.byref(Lo), s, _stream_ptr(q)))
+        ref = ctypes.byref
+        ws, ws_bytes = _workspace(workspace, lib().wha_packed_bwd_workspace_size(ref(Lq)), q)
+        _call("wha_packed_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr(),
+              lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_seqlens.data_ptr(), n_seq, code,
+              ws.data_ptr(), ws_bytes, ref(Lq), ref(Lk), ref(Lv), ref(Lo), s)
     return dq, dk, dv
 
 
@@ -630,29 +648,26 @@ def paged_kv_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     [n_pages][Hkv][page_size] (wha_paged_kv_write)."""
     Lk, Lv, code, ccode, pages, P = _paged_rows(k, v, slots, k_cache, v_cache, k_scale, v_scale)
     if k.numel() and pages:
-        with _on_device(k):
-            _check("wha_paged_kv_write", lib().wha_paged_kv_write(
-                _ptr(k), _ptr(v), _ptr(slots), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), code,
-                ccode, pages, P, ctypes.byref(Lk), ctypes.byref(Lv), _stream_ptr(k)))
+        _call("wha_paged_kv_write", k.device, k.data_ptr(), v.data_ptr(), slots.data_ptr(), k_cache.data_ptr(),
+              v_cache.data_ptr(), _address(k_scale), _address(v_scale), code, ccode, pages, P, ctypes.byref(Lk),
+              ctypes.byref(Lv))
 
 
 def paged_kv_read(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=None, out=None):
     """The rows of the slots out of a paged cache again (wha_paged_kv_read): (k, v)
     [N][Hkv][D] of `dtype` (the cache's own; for an int8 cache float32 unless
     given), zeros for negative slots.  out: a pair of views to write to."""
-    torch = _torch()
     if out is None:
         if dtype is None:
-            dtype = torch.float32 if k_cache.dtype == torch.int8 else k_cache.dtype
+            dtype = _torch().float32 if k_cache.dtype == _torch().int8 else k_cache.dtype
         shape = (slots.numel(), k_cache.shape[1], k_cache.shape[3])
-        out = tuple(torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
+        out = (k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype))
     k, v = out
     Lk, Lv, code, ccode, pages, P = _paged_rows(k, v, slots, k_cache, v_cache, k_scale, v_scale)
     if k.numel():
-        with _on_device(k):
-            _check("wha_paged_kv_read", lib().wha_paged_kv_read(
-                _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(slots), _ptr(k), _ptr(v), code,
-                ccode, pages, P, ctypes.byref(Lk), ctypes.byref(Lv), _stream_ptr(k)))
+        _call("wha_paged_kv_read", k.device, k_cache.data_ptr(), v_cache.data_ptr(), _address(k_scale),
+              _address(v_scale), slots.data_ptr(), k.data_ptr(), v.data_ptr(), code, ccode, pages, P,
+              ctypes.byref(Lk), ctypes.byref(Lv))
     return k, v
 
 
@@ -670,22 +685,19 @@ def paged_decode_fwd(q, k_cache, v_cache, block_table, lengths, k_scale=None, v_
         raise ValueError(f"q {tuple(q.shape)}, a table of {tuple(block_table.shape)}, {lengths.numel()} lengths and a "
                          f"cache of head dim {D} do not belong together")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape:
         raise ValueError(f"out: expected shape {tuple(q.shape)}, got {tuple(out.shape)}")
     Lo = _heads_layout(out, "out", q, rows=False)
     code = _dtype_code(q.dtype, "q")
-    lse = _lse_out(lse, (Lq.B, Lq.H), q.device) if want_lse else None
+    lse = _lse_out(lse, (Lq.B, Lq.H), q) if want_lse else None
     if q.numel():
         s = default_scale(D) if scale is None else float(scale)
-        per = block_table.shape[1]
-        with _on_device(q):
-            ws, ws_bytes = _workspace(workspace, int(lib().wha_paged_decode_workspace_size(
-                ctypes.byref(Lq), HK, P, per)), q.device)
-            _check("wha_paged_decode", lib().wha_paged_decode(
-                _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_table),
-                block_table.stride(0), per, _ptr(lengths), _ptr(out), _ptr(lse), _ptr(ws), ws_bytes, code, ccode,
-                pages, P, HK, ctypes.byref(Lq), ctypes.byref(Lo), s, _stream_ptr(q)))
+        per, ref = block_table.shape[1], ctypes.byref
+        ws, ws_bytes = _workspace(workspace, lib().wha_paged_decode_workspace_size(ref(Lq), HK, P, per), q)
+        _call("wha_paged_decode", q.device, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _address(k_scale),
+              _address(v_scale), block_table.data_ptr(), block_table.stride(0), per, lengths.data_ptr(),
+              out.data_ptr(), _address(lse), _address(ws), ws_bytes, code, ccode, pages, P, HK, ref(Lq), ref(Lo), s)
     return (out, lse) if want_lse else out
 
 

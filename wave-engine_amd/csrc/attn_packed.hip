@@ -90,101 +90,138 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
   return p;
 }
 
-// A tile of rows into LDS, ROWS x DP by NT threads.  VEC: direct-to-LDS buffer loads
-// from `base`, the address of the tile's first row, complete after wait_vmem: a
-// lane's offsets stay the same from tile to tile, and what moves is the descriptor,
-// in scalar registers.  Offsets past its range read as zeros: rows behind the last
-// one, and quads past the head dim.
+// The LDS tiles that the products read.
+template <class T, int DP, int ROWS>
+using Tile = typename std::conditional<sizeof(T) == 4, SplitTile<DP, ROWS>, LdsTile<T, DP>>::type;
+
+// A tile of rows from memory into LDS, ROWS x DP by NT threads, in two halves: begin
+// (the loads) and end (what is left to do when they are there).  off(rr): byte
+// offset of tile row rr in the range of the descriptor, past which is zero: rows
+// behind the last one, and what lies past the head dim.  What moves from tile to
+// tile is the descriptor, in scalar registers.
+// A: alignment of rows in bytes.  16-bit types: 16 or 4 bytes at a time straight to
+// LDS (complete after wait_vmem), or one element at a time (2).  float: 16 or 4
+// bytes at a time to registers, split on the way to LDS.
 constexpr int kPast = (int)0x80000000;
-template <class T, int DP, int ROWS, int NT>
+template <class T, int DP, int ROWS, int NT, int A>
 struct Stage {
-  using L = LdsTile<T, DP>;
-  static constexpr int PER = ROWS * L::kQuads / NT, Q = Elem<T>::kQuad;
-  static_assert(ROWS * L::kQuads % NT == 0, "whole rounds");
-  __device__ __forceinline__ static int row(int p, int tid) { return (p * NT + tid) / L::kQuads; }
-  __device__ __forceinline__ static int quad(int p, int tid) {
-    return ((p * NT + tid) % L::kQuads) ^ L::swz(row(p, tid));
-  }
-  // byte offset of quad c of a row `off` elements from the base
-  __device__ __forceinline__ static int at(int64_t off, int c, int D) {
-    return c * Q < D ? (int)((off + c * Q) * (int)sizeof(T)) : kPast;
-  }
-  __device__ __forceinline__ static void dma(__amdgpu_buffer_rsrc_t r, int off, char* lds, int p, int tid) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        r, (void __attribute__((address_space(3)))*)(lds + (p * NT + (tid & ~63)) * 16), 16, off, 0, 0, 0);
-  }
-  // one element at a time, from the row at `src`
-  __device__ __forceinline__ static void copy(const T* src, char* lds, int p, int tid, int D) {
-    const int c = quad(p, tid);
-    T x[Q];
+  using L = Tile<T, DP, ROWS>;
+  static constexpr int kRow = DP * (int)sizeof(T);  // bytes of a row in memory, padded
+  static constexpr int UNIT = sizeof(T) == 2 && A == 4 ? 4 : 16, UPR = kRow / UNIT, PER = ROWS * UPR / NT;
+  static_assert(ROWS * UPR % NT == 0, "whole rounds");
+  floatx4 x[sizeof(T) == 4 ? PER : 1];
+
+  template <class Off>
+  __device__ __forceinline__ void begin(__amdgpu_buffer_rsrc_t r, char* lds, int D, int tid, Off&& off) {
+    pin(tid);
 #pragma unroll
-    for (int e = 0; e < Q; ++e) x[e] = c * Q + e < D ? src[c * Q + e] : (T)0.f;
-    uintx4 y;
-    __builtin_memcpy(&y, x, 16);
-    *reinterpret_cast<uintx4*>(lds + (p * NT + tid) * 16) = y;
+    for (int p = 0; p < PER; ++p) {
+      const int i = p * NT + tid, rr = i / UPR, u = i % UPR;
+      if constexpr (sizeof(T) == 4) {
+        const int o = off(rr) + 16 * u;
+        if constexpr (A == 16) {
+          x[p] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, 4 * u < D ? o : kPast, 0, 0));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[p][e] = buffer_load_float(r, 4 * u + e < D ? o + 4 * e : kPast, 0);
+        }
+      } else {
+        // unit u of the row in LDS holds elements d .. of the row in memory
+        const int d = UNIT == 16 ? 8 * (u ^ L::swz(rr)) : 8 * ((u >> 2) ^ L::swz(rr)) + 2 * (u & 3);
+        const int o = off(rr) + 2 * d;
+        if constexpr (A == 2) {
+          unsigned short y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_raw_buffer_load_b16(r, d + e < D ? o + 2 * e : kPast, 0, 0);
+          uintx4 q;
+          __builtin_memcpy(&q, y, 16);
+          *reinterpret_cast<uintx4*>(lds + i * 16) = q;
+        } else {
+          auto* to = (void __attribute__((address_space(3)))*)(lds + (p * NT + (tid & ~63)) * UNIT);
+          if constexpr (UNIT == 16)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to, 16, d < D ? o : kPast, 0, 0, 0);
+          else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to, 4, d < D ? o : kPast, 0, 0, 0);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void end(char* lds, int tid) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const int i = p * NT + tid;
+        L::put4(lds, i / UPR, i % UPR, x[p]);
+      }
+    }
   }
   // rows row0 .. of one head, st elements apart, n of them in all
-  struct Lanes {
-    int off[PER];
-  };
-  template <bool VEC>
-  __device__ __forceinline__ static void lanes(Lanes& l, int64_t st, int D, int tid) {
-    if constexpr (VEC) {
-#pragma unroll
-      for (int p = 0; p < PER; ++p) l.off[p] = at(row(p, tid) * st, quad(p, tid), D);
-    }
-  }
-  template <bool VEC>
-  __device__ __forceinline__ static void head(const Lanes& l, const T* base, int row0, int n, int64_t st, int D,
-                                              char* lds, int tid) {
-    if constexpr (VEC) {
-      const int64_t left = ((int64_t)(min(n - row0, ROWS) - 1) * st + D) * (int64_t)sizeof(T);
-      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(base + (int64_t)row0 * st, (uint32_t)left);
-#pragma unroll
-      for (int p = 0; p < PER; ++p) dma(r, l.off[p], lds, p, tid);
-    } else {
-#pragma unroll
-      for (int p = 0; p < PER; ++p) copy(base + (int64_t)min(row0 + row(p, tid), n - 1) * st, lds, p, tid, D);
-    }
+  __device__ __forceinline__ void begin_head(const T* base, int row0, int n, int64_t st, char* lds, int D, int tid) {
+    const int64_t left = ((int64_t)(min(n - row0, ROWS) - 1) * st + D) * (int64_t)sizeof(T);
+    begin(buffer_rsrc(base + (int64_t)row0 * st, (uint32_t)left), lds, D, tid,
+          [&](int rr) { return rr * (int)st * (int)sizeof(T); });
   }
 };
 
-// d = 16 ks + 8 g .. + 7 of one row as a fragment (zero past the head dim).
-template <class T, bool VEC>
-__device__ __forceinline__ typename Elem<T>::Frag row_frag(const T* row, int ks, int g, int D) {
-  const int c = 16 * ks + 8 * g;
-  float x[8];
-  if constexpr (VEC && sizeof(T) == 2) {
+// Elements c .. c + 7 of one row (zero past the head dim).
+template <class T, int A>
+__device__ __forceinline__ typename Elem<T>::Frag row8(const T* row, int c, int D) {
+  if constexpr (A == 16 && sizeof(T) == 2) {
     uintx4 q = {0u, 0u, 0u, 0u};
     if (c < D) q = *reinterpret_cast<const uintx4*>(row + c);
     return __builtin_bit_cast(typename Elem<T>::Frag, q);
-  } else if constexpr (VEC) {
+  } else if constexpr (A == 4 && sizeof(T) == 2) {
+    uintx4 q = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      floatx4 q = {0.f, 0.f, 0.f, 0.f};
-      if (c + 4 * h < D) q = *reinterpret_cast<const floatx4*>(row + c + 4 * h);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * h + e] = q[e];
-    }
+    for (int i = 0; i < 4; ++i)
+      if (c + 2 * i < D) q[i] = *reinterpret_cast<const unsigned*>(row + c + 2 * i);
+    return __builtin_bit_cast(typename Elem<T>::Frag, q);
   } else {
+    float x[8];
+    if constexpr (A == 16) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = c + j < D ? (float)row[c + j] : 0.f;
+      for (int h = 0; h < 2; ++h) {
+        floatx4 q = {0.f, 0.f, 0.f, 0.f};
+        if (c + 4 * h < D) q = *reinterpret_cast<const floatx4*>(row + c + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * h + e] = q[e];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = c + j < D ? (float)row[c + j] : 0.f;
+    }
+    return Elem<T>::pack(x);
   }
-  return Elem<T>::pack(x);
+}
+template <class T>
+__device__ __forceinline__ typename Fast<T>::Frag fast_of(const typename Elem<T>::Frag& f) {
+  if constexpr (sizeof(T) == 4) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = f[j];
+    return Fast<T>::pack(x);
+  } else {
+    return f;
+  }
 }
 
 // Writes a lane's part of X^T[d][row] (d = 32 dt + row32(i, g)) to its row.
-template <class T, int NDT, bool VEC>
+template <class T, int NDT, int A>
 __device__ __forceinline__ void store_row(T* dst, int D, int g, const floatx16 (&x)[NDT], float mul) {
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int c = 32 * dt + 8 * u + 4 * g;
-      if constexpr (VEC) {
+      if constexpr (A == 16) {
         if (c < D)
           Elem<T>::store4(dst + c, x[dt][4 * u] * mul, x[dt][4 * u + 1] * mul, x[dt][4 * u + 2] * mul,
                           x[dt][4 * u + 3] * mul);
+      } else if constexpr (A == 4 && sizeof(T) == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+          if (c + e < D)
+            *reinterpret_cast<unsigned*>(dst + c + e) = Elem<T>::pair(x[dt][4 * u + e] * mul, x[dt][4 * u + e + 1] * mul);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -212,59 +249,76 @@ struct Frags {
   F f[N];
 };
 
-// Whether a tile holds an infinity or NaN (one wave looks at all of it).
-template <class T, int DP, int ROWS>
-__device__ __forceinline__ bool tile_not_finite(const char* t, int lane) {
-  unsigned bad = 0;
-#pragma unroll 1
-  for (int i = lane; i < ROWS * LdsTile<T, DP>::kQuads; i += 64) {
-    const uintx4 q = *reinterpret_cast<const uintx4*>(t + 16 * i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) bad |= not_finite_bits<T>(q[e]);
-  }
-  return __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-}
-
-// acc[d][column] += sum over the tile's rows of p[row][column] x[row][d]; weights of
-// rows that do not belong to a column are zero.
-template <class T, int DP, int NDT, int NSUB>
+// acc[d][column] += sum over the tile's 32 NSUB rows of p[row][column] x[row][d].
+template <class T, class L, int NDT, int NSUB>
 __device__ __forceinline__ void add_cols(const char* t, const floatx16 (&p)[NSUB], floatx16 (&acc)[NDT], int lane) {
-  typename Elem<T>::Frag f[2 * NSUB];
+  constexpr int N = 2 * NSUB;
+  typename Fast<T>::Frag f[N];
 #pragma unroll
-  for (int s = 0; s < 2 * NSUB; ++s) {
+  for (int s = 0; s < N; ++s) {
     float x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = p[s / 2][8 * (s & 1) + j];
-    f[s] = Elem<T>::pack(x);
+    f[s] = Fast<T>::pack(x);
   }
-  one_ahead<2 * NSUB * NDT>([&](int i) { return LdsTile<T, DP>::cols32(t, i / NDT, i % NDT, lane); },
-                            [&](int i, const typename Elem<T>::Frag& x) {
-                              acc[i % NDT] = Elem<T>::mma32(x, f[i / NDT], acc[i % NDT]);
-                            });
+  auto cols = [&](int i) { return L::cols32(t, i % N, i / N, lane); };
+  if constexpr (sizeof(T) == 4) {
+    typename Fast<T>::Sum sum;
+    one_ahead<N * NDT>(cols, [&](int i, const typename Fast<T>::Frag& x) {
+      if (i % N == 0) sum = typename Fast<T>::Sum();
+      sum.add(x, f[i % N]);
+      if (i % N == N - 1) {
+        const floatx16 y = sum.value();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i / N][e] += y[e];
+      }
+    });
+  } else {
+    one_ahead<N * NDT>(cols, [&](int i, const typename Fast<T>::Frag& x) {
+      acc[i / N] = Elem<T>::mma32(x, f[i % N], acc[i / N]);
+    });
+  }
 }
 
-// A weight of zero does not undo an infinity or NaN (0 x inf).  So where the mask
-// cuts through a tile that holds one, a wave leaves that tile's products and those
-// of the cut tiles after it out of its loop, and forms them here at the end: the
-// scores once more from memory, then row by row over the rows the mask leaves.  At
-// the end, because a second form of the products inside the loop costs the whole
-// kernel 60 registers and more.
-//
-// x y^T of 32 rows of memory each, by lane % 32.
-template <class T, int NKS, bool VEC>
+// Results that are not finite are formed once more, from memory, by the wave alone:
+// a weight of zero does not undo an infinity or NaN in the tiles that the mask cuts
+// through (0 x inf), and the split of fp32 knows no infinity.  Here scores and
+// products are Elem's, and the rows of a cut tile are added one by one, those only
+// that the mask leaves.  32 rows at a time, x y^T by lane % 32:
+template <class T, int NKS, int A>
 __device__ __forceinline__ floatx16 scores_of(const T* x, const T* y, int g, int D) {
   floatx16 s = zeros16();
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) {
-    s = Elem<T>::mma32(row_frag<T, VEC>(x, ks, g, D), row_frag<T, VEC>(y, ks, g, D), s);
+    s = Elem<T>::mma32(row8<T, A>(x, 16 * ks + 8 * g, D), row8<T, A>(y, 16 * ks + 8 * g, D), s);
     WHA_FENCE();
   }
   return s;
 }
-// acc[d][column] += p[row][column] row(x)[d] over the rows x with mine(x), of 32, the
-// weights by way of `w` (32 x 32 of the wave's own LDS).
+// acc[d][column] += p[row][column] row(x)[d] over 32 rows.
+template <class T, int NDT, class Row>
+__device__ __forceinline__ void add_all(const floatx16& p, floatx16 (&acc)[NDT], int lane, int D, Row&& row) {
+  const int g = lane >> 5, c = lane & 31;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = p[8 * s + j];
+    const typename Elem<T>::Frag f = Elem<T>::pack(y);
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 32 * dt + c < D ? (float)row(16 * s + row32(j, g))[32 * dt + c] : 0.f;
+      acc[dt] = Elem<T>::mma32(Elem<T>::pack(x), f, acc[dt]);
+      WHA_FENCE();
+    }
+  }
+}
+// The same over the rows with mine(x) only, the weights by way of `w` (32 x 32 of the
+// wave's own LDS).
 template <class T, int NDT, class Row, class Mine>
-__device__ __forceinline__ void add_rows(const floatx16& p, floatx16 (&acc)[NDT], T* w, int lane, int D, Row&& row,
+__device__ __forceinline__ void add_mine(const floatx16& p, floatx16 (&acc)[NDT], T* w, int lane, int D, Row&& row,
                                          Mine&& mine) {
   const int g = lane >> 5, c = lane & 31;
 #pragma unroll
@@ -287,37 +341,150 @@ __device__ __forceinline__ void add_rows(const floatx16& p, floatx16 (&acc)[NDT]
   }
   __builtin_amdgcn_wave_barrier();
 }
-
-}  // namespace
-
-// Whether a result of any wave of the block is not finite (bad: of this lane).
-__device__ __forceinline__ bool any_bad(bool bad, int* flags, int wave, int lane) {
-  const uint64_t some = __builtin_amdgcn_ballot_w64(bad);
-  if (lane == 0) flags[wave] = some != 0;
-  __syncthreads();
-  return (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
-}
+// Whether any lane's `on` results are not all finite.
 template <int NDT>
-__device__ __forceinline__ bool not_finite(const floatx16 (&x)[NDT]) {
+__device__ __forceinline__ bool any_not_finite(const floatx16 (&x)[NDT], bool on) {
   float chk = 0.f;  // NaN if any is not finite
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) chk = fmaf(x[dt][i], 0.f, chk);
-  return chk != 0.f;
+  return __builtin_amdgcn_ballot_w64(on && chk != 0.f) != 0;
 }
 
+// The tiles that the mask leaves whole first, then the cut ones, in loops of their own:
+// both forms of the sums in one loop would hold them twice.
+//
+// 32 rows of the forward: the maximum of each first (a running one would meet -inf -
+// -inf), then weights and O.
+template <class T, int NKS, int NDT, int A>
+__device__ __forceinline__ void fwd_again(const T* Qr, const T* Kb, const T* Vb, T* Or, float* lse_at, T* w,
+                                                    int64_t k_st, int64_t v_st, int len, int D, bool on, int t,
+                                                    int t_first, int t_last, float sl2, int lane) {
+  const int g = lane >> 5;
+  auto scores = [&](int k0) {
+    floatx16 s = scores_of<T, NKS, A>(Kb + (int64_t)min(k0 + (lane & 31), len - 1) * k_st, Qr, g, D);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = k0 + row32(i, g) > t ? -INFINITY : s[i];
+    return s;
+  };
+  float m = -INFINITY, l = 0.f;
+  floatx16 o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) o[dt] = zeros16();
+#pragma unroll 1
+  for (int k0 = 0; k0 <= t_last; k0 += 32) {
+    const floatx16 s = scores(k0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = vmax2(m, s[i]);
+  }
+  m = pair_max32(m) * sl2;
+  const float sub = m == -INFINITY ? 0.f : m;
+  auto weights = [&](int k0) {
+    floatx16 s = scores(k0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = fast_exp2(fmaf(s[i], sl2, -sub));
+      l += s[i];
+    }
+    return s;
+  };
+  int k0 = 0;
+  auto row = [&](int x) { return Vb + (int64_t)min(k0 + x, len - 1) * v_st; };
+#pragma unroll 1
+  for (; k0 + 31 <= t_first; k0 += 32) add_all<T>(weights(k0), o, lane, D, row);
+#pragma unroll 1
+  for (; k0 <= t_last; k0 += 32) add_mine<T>(weights(k0), o, w, lane, D, row, [&](int x) { return k0 + x <= t; });
+  l = pair_sum32(l);
+  if (on) {
+    store_row<T, NDT, A>(Or, D, g, o, 1.f / l);
+    if (lse_at != nullptr && g == 0) *lse_at = fmaf(m, kLn2, logf(l));
+  }
+}
+template <class T, int NKS, int NDT, int A>
+__device__ __forceinline__ void dq_again(const T* Qr, const T* Kb, const T* Vb, const T* DOr, T* dq_at, T* w,
+                                                   int64_t k_st, int64_t v_st, int len, int D, bool on, int t,
+                                                   int t_first, int t_last, float sl2, float lse2, float delta,
+                                                   float scale, int lane) {
+  const int g = lane >> 5;
+  floatx16 dq[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dq[dt] = zeros16();
+  int k0 = 0;
+  auto row = [&](int x) { return Kb + (int64_t)min(k0 + x, len - 1) * k_st; };
+  auto weights = [&]() {
+    floatx16 s = scores_of<T, NKS, A>(row(lane & 31), Qr, g, D);
+    const floatx16 dp = scores_of<T, NKS, A>(Vb + (int64_t)min(k0 + (lane & 31), len - 1) * v_st, DOr, g, D);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], sl2, -lse2)) * (dp[i] - delta);
+    return s;
+  };
+#pragma unroll 1
+  for (; k0 + 31 <= t_first; k0 += 32) add_all<T>(weights(), dq, lane, D, row);
+#pragma unroll 1
+  for (; k0 <= t_last; k0 += 32) add_mine<T>(weights(), dq, w, lane, D, row, [&](int x) { return k0 + x <= t; });
+  if (on) store_row<T, NDT, A>(dq_at, D, g, dq, scale);
+}
+// dK (KEYS) or dV of 32 keys; lse2, delta: the statistics of the group's rows.
+template <class T, int NKS, int NDT, int A, bool KEYS>
+__device__ __forceinline__ void dkv_again(const T* Qb, const T* Kr, const T* Vr, const T* Db, const float* lse2,
+                                          const float* delta, T* to, T* w, int64_t q_st, int64_t q_sh, int64_t o_st,
+                                          int64_t o_sh, int total, int G, int D, int rows, int key0, bool on,
+                                          float sl2, float scale, int lane) {
+  const int g = lane >> 5, first = (key0 + (lane & 31)) * G;
+  floatx16 acc[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) acc[dt] = zeros16();
+  int r0 = 0;
+  auto q_row = [&](int y) {
+    const int r = min(r0 + y, rows - 1);
+    return Qb + (int64_t)(r / G) * q_st + (int64_t)(r % G) * q_sh;
+  };
+  auto do_row = [&](int y) {
+    const int r = min(r0 + y, rows - 1);
+    return Db + (int64_t)(r / G) * o_st + (int64_t)(r % G) * o_sh;
+  };
+  auto row = [&](int y) { return KEYS ? q_row(y) : do_row(y); };
+  auto mine = [&](int y) { return r0 + y >= first && r0 + y < rows; };
+  auto weights = [&]() {
+    floatx16 p = scores_of<T, NKS, A>(q_row(lane & 31), Kr, g, D), dp = zeros16();
+    if constexpr (KEYS) dp = scores_of<T, NKS, A>(do_row(lane & 31), Vr, g, D);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = min(r0 + row32(i, g), rows - 1);
+      const int64_t at = (int64_t)(r % G) * total + r / G;
+      p[i] = fast_exp2(fmaf(p[i], sl2, -lse2[at]));
+      if constexpr (KEYS) p[i] *= dp[i] - delta[at];
+      if (i % 4 == 3) WHA_FENCE();
+    }
+    return p;
+  };
+  const int begin = key0 * G & ~31, whole = ((key0 + 31) * G + 31) & ~31;  // sub-tiles from `whole` on are not cut
+#pragma unroll 1
+  for (r0 = whole; r0 + 32 <= rows; r0 += 32) add_all<T>(weights(), acc, lane, D, row);
+  const int last = max(r0, whole);  // the one that the sequence's end cuts
+#pragma unroll 1
+  for (r0 = begin; r0 < rows; r0 = r0 + 32 < whole ? r0 + 32 : r0 < whole ? last : rows)
+    add_mine<T>(weights(), acc, w, lane, D, row, mine);
+  if (on) store_row<T, NDT, A>(to, D, g, acc, scale);
+}
+
+// Waves to a SIMD that the kernels' loops leave room for in its registers (fp32: three
+// parts of two operands and a result of 128 fill them).
+constexpr int waves_per_simd(int size, int ndt) { return size == 4 && ndt > 2 ? 1 : 2; }
+
+}  // namespace
+
 // ---------------------------------------------------------------- forward
-template <class T, int NKS, int NDT, bool VEC>
-__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict__ Q, const T* __restrict__ K,
-                                                            const T* __restrict__ V, T* __restrict__ O,
-                                                            float* __restrict__ LSE, PackedArgs a, float sl2) {
+template <class T, int NKS, int NDT, int A>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && NDT <= 2 ? 3 : waves_per_simd(sizeof(T), NDT)) void packed_fwd_kernel(
+    const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, T* __restrict__ O,
+    float* __restrict__ LSE, PackedArgs a, float sl2) {
   constexpr int DP = 32 * NDT, NT = 256, BM = 128, KT = sizeof(T) == 4 ? 32 : 64, NSUB = KT / 32;
-  using L = LdsTile<T, DP>;
-  using St = Stage<T, DP, KT, NT>;
+  using L = Tile<T, DP, KT>;
+  using F = Fast<T>;
   constexpr int BYTES = KT * L::kRow;
   __shared__ __align__(16) char K0[BYTES], K1[BYTES], V0[BYTES], V1[BYTES];
-  __shared__ int flags[4];
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -329,40 +496,43 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
   const int r = r0 + (lane & 31), rc = min(r, rows - 1), t = rc / G, h = hk * G + rc % G;
   const T* Kb = K + (int64_t)pl.start * a.k_st + (int64_t)hk * a.k_sh;
   const T* Vb = V + (int64_t)pl.start * a.v_st + (int64_t)hk * a.v_sh;
-  typename St::Lanes kl, vl;
-  St::template lanes<VEC>(kl, a.k_st, D, tid);
-  St::template lanes<VEC>(vl, a.v_st, D, tid);
-  auto stage_kv = [&](int kt, char* Kd, char* Vd) {
-    St::template head<VEC>(kl, Kb, kt * KT, pl.len, a.k_st, D, Kd, tid);
-    St::template head<VEC>(vl, Vb, kt * KT, pl.len, a.v_st, D, Vd, tid);
+  Stage<T, DP, KT, NT, A> ks_, vs_;
+  auto begin = [&](int kt, char* Kd, char* Vd) {
+    ks_.begin_head(Kb, kt * KT, pl.len, a.k_st, Kd, D, tid);
+    vs_.begin_head(Vb, kt * KT, pl.len, a.v_st, Vd, D, tid);
+  };
+  auto end = [&](char* Kd, char* Vd) {
+    ks_.end(Kd, tid);
+    vs_.end(Vd, tid);
   };
   const int n_kt = min(pl.tile * BM + BM - 1, rows - 1) / G / KT + 1;  // tiles that the block sweeps
   const int t_first = __builtin_amdgcn_readfirstlane(t), t_last = __builtin_amdgcn_readlane(t, 31);
   const int n_w = r0 < rows ? t_last / KT + 1 : 0;  // tiles with a key before some query of the wave
-  stage_kv(0, K0, V0);
+  begin(0, K0, V0);
 
-  typename Elem<T>::Frag qf[NKS];
+  typename F::Frag qf[NKS];
   const T* Qr = Q + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh;
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) qf[ks] = row_frag<T, VEC>(Qr, ks, g, D);
+  for (int ks = 0; ks < NKS; ++ks) qf[ks] = fast_of<T>(row8<T, A>(Qr, 16 * ks + 8 * g, D));
+  end(K0, V0);
 
-  float m, l;  // running maximum (log2 units), this lane's part of the row sum
+  float m = -INFINITY, l = 0.f;  // running maximum (log2 units), this lane's part of the row sum
   floatx16 o[NDT];
-  bool check = false;
-  int left;  // the first cut tile left to the end
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) o[dt] = zeros16();
   auto tile = [&](int kt, const char* Kt, const char* Vt) {
     const int k0 = kt * KT;
     int ln = lane;
     pin(ln);
     floatx16 s[NSUB];
-#pragma unroll
-    for (int x = 0; x < NSUB; ++x) s[x] = zeros16();
+    typename F::Sum sum;
     one_ahead<NSUB * NKS>([&](int i) { return L::rows32(Kt, 32 * (i / NKS), i % NKS, ln); },
-                          [&](int i, const typename Elem<T>::Frag& f) {
-                            s[i / NKS] = Elem<T>::mma32(f, qf[i % NKS], s[i / NKS]);
+                          [&](int i, const typename F::Frag& f) {
+                            if (i % NKS == 0) sum = typename F::Sum();
+                            sum.add(f, qf[i % NKS]);
+                            if (i % NKS == NKS - 1) s[i / NKS] = sum.value();
                           });
-    const bool cut = k0 + KT - 1 > t_first;  // wave-uniform: the mask cuts through the tile
-    if (cut) {
+    if (k0 + KT - 1 > t_first) {  // wave-uniform: the mask cuts through the tile
 #pragma unroll
       for (int x = 0; x < NSUB; ++x)
 #pragma unroll
@@ -394,65 +564,50 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(const T* __restrict_
         s[x][i] = fast_exp2(fmaf(s[x][i], sl2, -sub));
         l += s[x][i];
       }
-    if (check && cut && kt < left && tile_not_finite<T, DP, KT>(Vt, lane)) left = kt;
-    if (kt < left) add_cols<T, DP>(Vt, s, o, ln);
+    add_cols<T, L>(Vt, s, o, ln);
   };
   auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
-    if constexpr (VEC) wait_vmem();
+    if constexpr (sizeof(T) == 2) wait_vmem();
     __syncthreads();  // tile kt is in LDS; every wave is done with the other buffers
-    if (kt + 1 < n_kt) stage_kv(kt + 1, Kn, Vn);
+    if (kt + 1 < n_kt) begin(kt + 1, Kn, Vn);
     if (kt < n_w) tile(kt, Kt, Vt);
+    if (kt + 1 < n_kt) end(Kn, Vn);
   };
-  for (;;) {
-    m = -INFINITY, l = 0.f, left = n_w;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[dt] = zeros16();
-    for (int kt = 0; kt < n_kt; kt += 2) {
-      step(kt, K0, V0, K1, V1);
-      if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
-    }
-    // an infinity or NaN: once more, with an eye on the tiles that the mask cuts
-    if (check || !any_bad(r < rows && not_finite(o), flags, wave, lane)) break;
-    check = true;
-    stage_kv(0, K0, V0);
-  }
-  if (check) {
-    __syncthreads();  // the tiles' LDS is free
-    T* w = reinterpret_cast<T*>(wave & 2 ? K1 : K0) + (wave & 1) * 1024;
-    for (int k0 = left * KT; k0 < n_w * KT; k0 += 32) {
-      floatx16 s = scores_of<T, NKS, VEC>(Kb + (int64_t)min(k0 + (lane & 31), pl.len - 1) * a.k_st, Qr, g, D);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], sl2, -(m == -INFINITY ? 0.f : m)));
-      add_rows<T>(
-          s, o, w, lane, D, [&](int x) { return Vb + (int64_t)min(k0 + x, pl.len - 1) * a.v_st; },
-          [&](int x) { return k0 + x <= t; });
-    }
+  for (int kt = 0; kt < n_kt; kt += 2) {
+    step(kt, K0, V0, K1, V1);
+    if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
   }
   l = pair_sum32(l);
-  if (r < rows) {
-    store_row<T, NDT, VEC>(O + (int64_t)(pl.start + t) * a.o_st + (int64_t)h * a.o_sh, D, g, o, 1.f / l);
-    if (LSE != nullptr && g == 0) LSE[(int64_t)h * a.total + pl.start + t] = fmaf(m, kLn2, logf(l));
+  __syncthreads();  // the tiles' LDS is free
+  T* Or = O + (int64_t)(pl.start + t) * a.o_st + (int64_t)h * a.o_sh;
+  float* lse_at = LSE == nullptr ? nullptr : LSE + (int64_t)h * a.total + pl.start + t;
+  if (any_not_finite(o, r < rows)) {
+    fwd_again<T, NKS, NDT, A>(Qr, Kb, Vb, Or, lse_at, reinterpret_cast<T*>(wave & 2 ? K1 : K0) + (wave & 1) * 1024,
+                              a.k_st, a.v_st, pl.len, D, r < rows, t, t_first, t_last, sl2, lane);
+  } else if (r < rows) {
+    store_row<T, NDT, A>(Or, D, g, o, 1.f / l);
+    if (lse_at != nullptr && g == 0) *lse_at = fmaf(m, kLn2, logf(l));
   }
 }
 
 // ---------------------------------------------------------------- backward
-// (fp32 rows of 128 fill a wave's registers with two operands and a result: one
-// wave to a SIMD, without spills)
-constexpr int waves_per_simd(int size, int ndt) { return size == 4 && ndt > 2 ? 1 : 2; }
-
 // Query-stationary: dQ, and the row statistics lse log2(e) and Delta that the
 // key-stationary kernel reads.
-template <class T, int NKS, int NDT, bool VEC>
+//
+// Delta = do . o takes o as the forward rounded it; in 16 bits the error is as large
+// as that of the rounded score gradients where a row has few keys.  Blocks whose
+// rows all lie below kShort sum Delta over p dp in a sweep of its own instead.
+constexpr int kShort = 256;
+template <class T, int NKS, int NDT, int A>
 __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq_kernel(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ O,
     const T* __restrict__ DO, const float* __restrict__ LSE, T* __restrict__ DQ, float* __restrict__ LSE2,
     float* __restrict__ DELTA, PackedArgs a, float sl2, float scale) {
   constexpr int DP = 32 * NDT, NT = 256, BM = 128, KT = sizeof(T) == 4 ? 32 : 64, NSUB = KT / 32;
-  using L = LdsTile<T, DP>;
-  using St = Stage<T, DP, KT, NT>;
+  using L = Tile<T, DP, KT>;
+  using F = Fast<T>;
   constexpr int BYTES = KT * L::kRow;
   __shared__ __align__(16) char K0[BYTES], K1[BYTES], V0[BYTES], V1[BYTES];
-  __shared__ int flags[4];
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -463,41 +618,42 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
   const int r = r0 + (lane & 31), rc = min(r, rows - 1), t = rc / G, h = hk * G + rc % G;
   const T* Kb = K + (int64_t)pl.start * a.k_st + (int64_t)hk * a.k_sh;
   const T* Vb = V + (int64_t)pl.start * a.v_st + (int64_t)hk * a.v_sh;
-  typename St::Lanes kl, vl;
-  St::template lanes<VEC>(kl, a.k_st, D, tid);
-  St::template lanes<VEC>(vl, a.v_st, D, tid);
-  auto stage_kv = [&](int kt, char* Kd, char* Vd) {
-    St::template head<VEC>(kl, Kb, kt * KT, pl.len, a.k_st, D, Kd, tid);
-    St::template head<VEC>(vl, Vb, kt * KT, pl.len, a.v_st, D, Vd, tid);
+  Stage<T, DP, KT, NT, A> ks_, vs_;
+  auto begin = [&](int kt, char* Kd, char* Vd) {
+    ks_.begin_head(Kb, kt * KT, pl.len, a.k_st, Kd, D, tid);
+    vs_.begin_head(Vb, kt * KT, pl.len, a.v_st, Vd, D, tid);
   };
-  const int n_kt = min(pl.tile * BM + BM - 1, rows - 1) / G / KT + 1;
+  auto end = [&](char* Kd, char* Vd) {
+    ks_.end(Kd, tid);
+    vs_.end(Vd, tid);
+  };
+  const int t_end = min(pl.tile * BM + BM - 1, rows - 1) / G;
+  const int n_kt = t_end / KT + 1;
   const int t_first = __builtin_amdgcn_readfirstlane(t), t_last = __builtin_amdgcn_readlane(t, 31);
   const int n_w = r0 < rows ? t_last / KT + 1 : 0;
-  stage_kv(0, K0, V0);
+  begin(0, K0, V0);
 
-  typename Elem<T>::Frag qf[NKS], dof[NKS];
+  typename F::Frag qf[NKS], dof[NKS];
   const T* Qr = Q + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh;
   const int64_t o_at = (int64_t)(pl.start + t) * a.o_st + (int64_t)h * a.o_sh;
   const int64_t stat_at = (int64_t)h * a.total + pl.start + t;
   float delta = 0.f;
 #pragma unroll
   for (int ks = 0; ks < NKS; ++ks) {
-    qf[ks] = row_frag<T, VEC>(Qr, ks, g, D);
-    dof[ks] = row_frag<T, VEC>(DO + o_at, ks, g, D);
-    const typename Elem<T>::Frag of = row_frag<T, VEC>(O + o_at, ks, g, D);
+    qf[ks] = fast_of<T>(row8<T, A>(Qr, 16 * ks + 8 * g, D));
+    const typename Elem<T>::Frag d = row8<T, A>(DO + o_at, 16 * ks + 8 * g, D);
+    const typename Elem<T>::Frag of = row8<T, A>(O + o_at, 16 * ks + 8 * g, D);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) delta = fmaf((float)of[j], (float)dof[ks][j], delta);
+    for (int j = 0; j < 8; ++j) delta = fmaf((float)of[j], (float)d[j], delta);
+    dof[ks] = fast_of<T>(d);
   }
   delta = pair_sum32(delta);
   const float lse2 = LSE[stat_at] * kLog2e;
-  if (r < rows && g == 0) {
-    LSE2[stat_at] = lse2;
-    DELTA[stat_at] = delta;
-  }
+  end(K0, V0);
   floatx16 dq[NDT];
-  bool check = false;
-  int left;
-  auto tile = [&](int kt, const char* Kt, const char* Vt) {
+  float sum_delta = 0.f;
+  auto tile = [&](auto sums, int kt, const char* Kt, const char* Vt) {
+    constexpr bool SUMS = decltype(sums)::value;  // the sweep that sums Delta
     const int k0 = kt * KT;
     int ln = lane;
     pin(ln);
@@ -505,78 +661,90 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
     const bool cut = k0 + KT - 1 > t_first;
 #pragma unroll
     for (int x = 0; x < NSUB; ++x) {
-      floatx16 s = zeros16(), dp = zeros16();
-      typedef Frags<typename Elem<T>::Frag, 2> F2;
+      typename F::Sum s, dp;
+      typedef Frags<typename F::Frag, 2> F2;
       one_ahead<NKS>([&](int ks) { return F2{{L::rows32(Kt, 32 * x, ks, ln), L::rows32(Vt, 32 * x, ks, ln)}}; },
                      [&](int ks, const F2& f) {
-                       s = Elem<T>::mma32(f.f[0], qf[ks], s);
-                       dp = Elem<T>::mma32(f.f[1], dof[ks], dp);
+                       s.add(f.f[0], qf[ks]);
+                       dp.add(f.f[1], dof[ks]);
                      });
+      const floatx16 sv = s.value(), dv = dp.value();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) ds[x][i] = fast_exp2(fmaf(s[i], sl2, -lse2)) * (dp[i] - delta);
+      for (int i = 0; i < 16; ++i) {
+        const float p = fast_exp2(fmaf(sv[i], sl2, -lse2));
+        ds[x][i] = SUMS ? p * dv[i] : p * (dv[i] - delta);
+      }
       if (cut) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) ds[x][i] = k0 + 32 * x + row32(i, g) > t ? 0.f : ds[x][i];
       }
     }
-    if (check && cut && kt < left && tile_not_finite<T, DP, KT>(Kt, lane)) left = kt;
-    if (kt < left) add_cols<T, DP>(Kt, ds, dq, ln);
-  };
-  auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
-    if constexpr (VEC) wait_vmem();
-    __syncthreads();
-    if (kt + 1 < n_kt) stage_kv(kt + 1, Kn, Vn);
-    if (kt < n_w) tile(kt, Kt, Vt);
-  };
-  for (;;) {
-    left = n_w;
+    if constexpr (SUMS) {
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) dq[dt] = zeros16();
+      for (int x = 0; x < NSUB; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum_delta += ds[x][i];
+    } else {
+      add_cols<T, L>(Kt, ds, dq, ln);
+    }
+  };
+  auto sweep = [&](auto sums) {
+    auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
+      if constexpr (sizeof(T) == 2) wait_vmem();
+      __syncthreads();
+      if (kt + 1 < n_kt) begin(kt + 1, Kn, Vn);
+      if (kt < n_w) tile(sums, kt, Kt, Vt);
+      if (kt + 1 < n_kt) end(Kn, Vn);
+    };
     for (int kt = 0; kt < n_kt; kt += 2) {
       step(kt, K0, V0, K1, V1);
       if (kt + 1 < n_kt) step(kt + 1, K1, V1, K0, V0);
     }
-    if (check || !any_bad(r < rows && not_finite(dq), flags, wave, lane)) break;
-    check = true;
-    stage_kv(0, K0, V0);
-  }
-  if (check) {
     __syncthreads();
-    T* w = reinterpret_cast<T*>(wave & 2 ? K1 : K0) + (wave & 1) * 1024;
-    for (int k0 = left * KT; k0 < n_w * KT; k0 += 32) {
-      const int64_t key = min(k0 + (lane & 31), pl.len - 1);
-      floatx16 s = scores_of<T, NKS, VEC>(Kb + key * a.k_st, Qr, g, D);
-      const floatx16 dp = scores_of<T, NKS, VEC>(Vb + key * a.v_st, DO + o_at, g, D);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = fast_exp2(fmaf(s[i], sl2, -lse2)) * (dp[i] - delta);
-      add_rows<T>(
-          s, dq, w, lane, D, [&](int x) { return Kb + (int64_t)min(k0 + x, pl.len - 1) * a.k_st; },
-          [&](int x) { return k0 + x <= t; });
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (t_end < kShort) {
+      sweep(std::true_type{});
+      delta = pair_sum32(sum_delta);
+      begin(0, K0, V0);
     }
   }
-  if (r < rows)
-    store_row<T, NDT, VEC>(DQ + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh, D, g, dq, scale);
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dq[dt] = zeros16();
+  sweep(std::false_type{});
+  if (r < rows && g == 0) {
+    LSE2[stat_at] = lse2;
+    DELTA[stat_at] = delta;
+  }
+  T* dq_at = DQ + (int64_t)(pl.start + t) * a.q_st + (int64_t)h * a.q_sh;
+  if (any_not_finite(dq, r < rows))
+    dq_again<T, NKS, NDT, A>(Qr, Kb, Vb, DO + o_at, dq_at, reinterpret_cast<T*>(wave & 2 ? K1 : K0) + (wave & 1) * 1024,
+                             a.k_st, a.v_st, pl.len, D, r < rows, t, t_first, t_last, sl2, lse2, delta, scale, lane);
+  else if (r < rows)
+    store_row<T, NDT, A>(dq_at, D, g, dq, scale);
 }
 
 // Key-stationary: dK and dV of 32 KG keys, over the rows of the group that come
 // after them: KG waves of 32 keys each, times 4 / KG that take every other 32 rows
 // and are added up at the end (KG = 2: where blocks of 128 keys are too few for the
 // CUs).
-template <class T, int NKS, int NDT, int KG, bool VEC>
+template <class T, int NKS, int NDT, int KG, int A>
 __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dkv_kernel(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ DO,
     const float* __restrict__ LSE2, const float* __restrict__ DELTA, T* __restrict__ DK, T* __restrict__ DV,
     PackedArgs a, float sl2, float scale) {
   static_assert(KG == 4 || KG == 2, "one or two row groups");
   constexpr int DP = 32 * NDT, NT = 256, BN = 32 * KG, RG = 4 / KG, QT = 32 * RG;
-  using L = LdsTile<T, DP>;
-  using St = Stage<T, DP, QT, NT>;
-  using StV = Stage<T, DP, BN, NT>;
+  using L = Tile<T, DP, QT>;
+  using F = Fast<T>;
   constexpr int BYTES = QT * L::kRow;
+  // 16-bit: V of the block's keys in LDS, in registers it would not fit beside K, dK
+  // and dV of 128; fp32: in registers, LDS would hold fewer blocks
+  constexpr bool V_LDS = sizeof(T) == 2;
+  using LV = LdsTile<typename std::conditional<V_LDS, T, __bf16>::type, DP>;
   __shared__ __align__(16) char Q0[BYTES], Q1[BYTES], D0[BYTES], D1[BYTES];
   __shared__ __align__(16) float S0[2 * QT], S1[2 * QT];  // a tile's lse log2(e), then its Delta
-  __shared__ __align__(16) char VS[BN * L::kRow];  // V of the block's keys: in registers it would not fit beside K, dK, dV
-  __shared__ int flags[4];
+  __shared__ __align__(16) char VS[V_LDS ? BN * LV::kRow : 16];
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, G = a.G, D = a.D;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave % KG, rg = wave / KG;
@@ -593,78 +761,90 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
   // position and head of row rr of a tile (G <= 128: a 16-bit reciprocal is exact
   // below 512); rows behind the last one repeat it
   const int magic = 65535 / G + 1;
-  auto stage_q = [&](int rt, char* Qd, char* Dd, float* Sd) {
-    const int t0 = rt * QT / G, g0 = rt * QT % G, end = rows - 1 - rt * QT;
+  Stage<T, DP, QT, NT, A> qs_, ds_;
+  auto begin = [&](int rt, char* Qd, char* Dd, float* Sd) {
+    const int t0 = rt * QT / G, g0 = rt * QT % G, last = rows - 1 - rt * QT;
     auto place = [&](int rr, int& t, int& gq) {
-      const int x = min(rr, end) + g0;
+      const int x = min(rr, last) + g0;
       t = (x * magic) >> 16;
       gq = x - t * G;
     };
-    const T *q = Qb + (int64_t)t0 * a.q_st, *d = Db + (int64_t)t0 * a.o_st;
-#pragma unroll
-    for (int p = 0; p < St::PER; ++p) {
+    auto at = [&](int rr, int64_t st, int64_t sh) {
       int t, gq;
-      place(St::row(p, tid), t, gq);
-      if constexpr (VEC) {
-        const int c = St::quad(p, tid);
-        St::dma(buffer_rsrc(q, 0x7fffffffu), St::at((int)(t * a.q_st + gq * a.q_sh), c, D), Qd, p, tid);
-        St::dma(buffer_rsrc(d, 0x7fffffffu), St::at((int)(t * a.o_st + gq * a.o_sh), c, D), Dd, p, tid);
-      } else {
-        St::copy(q + t * a.q_st + gq * a.q_sh, Qd, p, tid, D);
-        St::copy(d + t * a.o_st + gq * a.o_sh, Dd, p, tid, D);
-      }
-    }
+      place(rr, t, gq);
+      return (t * (int)st + gq * (int)sh) * (int)sizeof(T);
+    };
+    qs_.begin(buffer_rsrc(Qb + (int64_t)t0 * a.q_st, 0x7fffffffu), Qd, D, tid,
+              [&](int rr) { return at(rr, a.q_st, a.q_sh); });
+    ds_.begin(buffer_rsrc(Db + (int64_t)t0 * a.o_st, 0x7fffffffu), Dd, D, tid,
+              [&](int rr) { return at(rr, a.o_st, a.o_sh); });
     if (wave < RG) {  // 64 of the 2 QT statistics to a wave
       int t, gq;
       place((wave * 64 + lane) % QT, t, gq);
-      const int64_t at = stat0 + (int64_t)gq * a.total + t0 + t;
-      dma_dword((wave * 64 + lane < QT ? LSE2 : DELTA) + at, Sd + wave * 64);
+      const int64_t i = stat0 + (int64_t)gq * a.total + t0 + t;
+      dma_dword((wave * 64 + lane < QT ? LSE2 : DELTA) + i, Sd + wave * 64);
     }
+  };
+  auto end = [&](char* Qd, char* Dd) {
+    qs_.end(Qd, tid);
+    ds_.end(Dd, tid);
   };
   const int rt0 = pl.tile * BN * G / QT, n_rt = (rows + QT - 1) / QT;
   // sub-tiles of 32 rows: the first with a row after some key of the wave
   const int sub0 = key0 < pl.len ? key0 * G / 32 : 0x7fffffff;
-  {
-    typename StV::Lanes vl;
-    StV::template lanes<VEC>(vl, a.v_st, D, tid);
-    StV::template head<VEC>(vl, Vb, pl.tile * BN, pl.len, a.v_st, D, VS, tid);
-  }
-  stage_q(rt0, Q0, D0, S0);
-  const char* Vw = VS + kg * 32 * L::kRow;
+  if constexpr (V_LDS) Stage<T, DP, BN, NT, A>().begin_head(Vb, pl.tile * BN, pl.len, a.v_st, VS, D, tid);
+  begin(rt0, Q0, D0, S0);
+  const char* Vw = VS + kg * 32 * LV::kRow;
 
-  typename Elem<T>::Frag kf[NKS];
+  typename F::Frag kf[NKS], vf[V_LDS ? 1 : NKS];
   const T* Kr = K + (int64_t)(pl.start + kc) * a.k_st + (int64_t)hk * a.k_sh;
+  const T* Vr = Vb + (int64_t)kc * a.v_st;
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) kf[ks] = row_frag<T, VEC>(Kr, ks, g, D);
+  for (int ks = 0; ks < NKS; ++ks) {
+    kf[ks] = fast_of<T>(row8<T, A>(Kr, 16 * ks + 8 * g, D));
+    if constexpr (!V_LDS) vf[ks] = fast_of<T>(row8<T, A>(Vr, 16 * ks + 8 * g, D));
+  }
+  end(Q0, D0);
   floatx16 dk[NDT], dv[NDT];
-  bool check = false;
-  int left;  // the first cut sub-tile left to the end
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dk[dt] = zeros16(), dv[dt] = zeros16();
   // the mask (or the sequence's end) cuts through sub-tile x
   auto is_cut = [&](int x) { return x * 32 < (key0 + 31) * G || x * 32 + 32 > rows; };
-  auto tile = [&](int rt, const char* Qt, const char* Dt, const float* St_) {
-    const int x = rt * RG + rg, r0 = x * 32;
+  auto tile = [&](int x, const char* Qt, const char* Dt, const float* St) {
+    const int r0 = x * 32;
     int ln = lane;
     pin(ln);
     floatx16 p[1], ds[1];
-    floatx16 s = zeros16(), dp = zeros16();
-    one_ahead<NKS>([&](int ks) { return L::rows32(Qt, 0, ks, ln); },
-                   [&](int ks, const typename Elem<T>::Frag& f) { s = Elem<T>::mma32(f, kf[ks], s); });
-    typedef Frags<typename Elem<T>::Frag, 2> F2;
-    one_ahead<NKS>([&](int ks) { return F2{{L::rows32(Dt, 0, ks, ln), L::rows32(Vw, 0, ks, ln)}}; },
-                   [&](int ks, const F2& f) { dp = Elem<T>::mma32(f.f[0], f.f[1], dp); });
-    const bool cut = is_cut(x);
+    {
+      typename F::Sum s;
+      one_ahead<NKS>([&](int ks) { return L::rows32(Qt, 0, ks, ln); },
+                     [&](int ks, const typename F::Frag& f) { s.add(f, kf[ks]); });
+      p[0] = s.value();
+    }
+    {
+      typename F::Sum s;
+      if constexpr (V_LDS) {
+        typedef Frags<typename F::Frag, 2> F2;
+        one_ahead<NKS>([&](int ks) { return F2{{L::rows32(Dt, 0, ks, ln), LV::rows32(Vw, 0, ks, ln)}}; },
+                       [&](int ks, const F2& f) { s.add(f.f[0], f.f[1]); });
+      } else {
+        one_ahead<NKS>([&](int ks) { return L::rows32(Dt, 0, ks, ln); },
+                       [&](int ks, const typename F::Frag& f) { s.add(f, vf[ks]); });
+      }
+      ds[0] = s.value();
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const floatx4 lse2 = *reinterpret_cast<const floatx4*>(St_ + 8 * u + 4 * g);
-      const floatx4 delta = *reinterpret_cast<const floatx4*>(St_ + QT + 8 * u + 4 * g);
+      const floatx4 lse2 = *reinterpret_cast<const floatx4*>(St + 8 * u + 4 * g);
+      const floatx4 delta = *reinterpret_cast<const floatx4*>(St + QT + 8 * u + 4 * g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * u + e;
-        p[0][i] = fast_exp2(fmaf(s[i], sl2, -lse2[e]));
-        ds[0][i] = p[0][i] * (dp[i] - delta[e]);
+        p[0][i] = fast_exp2(fmaf(p[0][i], sl2, -lse2[e]));
+        ds[0][i] = p[0][i] * (ds[0][i] - delta[e]);
       }
     }
-    if (cut) {
+    if (is_cut(x)) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int row = r0 + row32(i, g);
@@ -673,62 +853,24 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
         ds[0][i] = in ? ds[0][i] : 0.f;
       }
     }
-    if (check && cut && x < left && (tile_not_finite<T, DP, 32>(Qt, lane) || tile_not_finite<T, DP, 32>(Dt, lane)))
-      left = x;
-    if (!cut || x < left) {
-      add_cols<T, DP>(Dt, p, dv, ln);
-      add_cols<T, DP>(Qt, ds, dk, ln);
-    }
+    add_cols<T, L>(Dt, p, dv, ln);
+    add_cols<T, L>(Qt, ds, dk, ln);
   };
-  auto step = [&](int rt, char* Qt, char* Dt, float* St_, char* Qn, char* Dn, float* Sn) {
+  // rows 32 rg .. of a tile (fp32: of each of its parts)
+  const int own = rg * 32 * (V_LDS ? L::kRow : LV::kRow);
+  auto step = [&](int rt, char* Qt, char* Dt, float* St, char* Qn, char* Dn, float* Sn) {
     wait_vmem();
     __syncthreads();
-    if (rt + 1 < n_rt) stage_q(rt + 1, Qn, Dn, Sn);
+    if (rt + 1 < n_rt) begin(rt + 1, Qn, Dn, Sn);
     const int x = rt * RG + rg;
-    if (x >= sub0 && x * 32 < rows)
-      tile(rt, Qt + rg * 32 * L::kRow, Dt + rg * 32 * L::kRow, St_ + rg * 32);
+    if (x >= sub0 && x * 32 < rows) tile(x, Qt + own, Dt + own, St + rg * 32);
+    if (rt + 1 < n_rt) end(Qn, Dn);
   };
-  for (;;) {
-    left = 0x7fffffff;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) dk[dt] = zeros16(), dv[dt] = zeros16();
-    for (int rt = rt0; rt < n_rt; rt += 2) {
-      step(rt, Q0, D0, S0, Q1, D1, S1);
-      if (rt + 1 < n_rt) step(rt + 1, Q1, D1, S1, Q0, D0, S0);
-    }
-    if (check || !any_bad(key < pl.len && (not_finite(dk) || not_finite(dv)), flags, wave, lane)) break;
-    check = true;
-    stage_q(rt0, Q0, D0, S0);
+  for (int rt = rt0; rt < n_rt; rt += 2) {
+    step(rt, Q0, D0, S0, Q1, D1, S1);
+    if (rt + 1 < n_rt) step(rt + 1, Q1, D1, S1, Q0, D0, S0);
   }
   __syncthreads();  // the tiles' LDS is free
-  if (check && left != 0x7fffffff) {
-    T* w = reinterpret_cast<T*>(wave & 2 ? Q1 : Q0) + (wave & 1) * 1024;
-    const T* Vr = Vb + (int64_t)kc * a.v_st;
-    for (int x = left; x * 32 < rows; x += RG) {
-      if (!is_cut(x)) continue;
-      const int r0 = x * 32;
-      auto q_row = [&](int y) {
-        const int r = min(r0 + y, rows - 1);
-        return Qb + (int64_t)(r / G) * a.q_st + (int64_t)(r % G) * a.q_sh;
-      };
-      auto do_row = [&](int y) {
-        const int r = min(r0 + y, rows - 1);
-        return Db + (int64_t)(r / G) * a.o_st + (int64_t)(r % G) * a.o_sh;
-      };
-      auto mine = [&](int y) { return r0 + y >= first && r0 + y < rows; };
-      floatx16 p = scores_of<T, NKS, VEC>(q_row(lane & 31), Kr, g, D);
-      floatx16 ds = scores_of<T, NKS, VEC>(do_row(lane & 31), Vr, g, D);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = min(r0 + row32(i, g), rows - 1);
-        const int64_t at = stat0 + (int64_t)(r % G) * a.total + r / G;
-        p[i] = fast_exp2(fmaf(p[i], sl2, -LSE2[at]));
-        ds[i] = p[i] * (ds[i] - DELTA[at]);
-      }
-      add_rows<T>(p, dv, w, lane, D, do_row, mine);
-      add_rows<T>(ds, dk, w, lane, D, q_row, mine);
-    }
-  }
   if constexpr (RG == 2) {  // the second row group's sums by way of LDS: dK in Q0 or Q1, dV in D0 or D1
     __syncthreads();
     float* k_sum = reinterpret_cast<float*>(kg ? Q1 : Q0) + lane;
@@ -753,27 +895,36 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
         dv[dt][i] += v_sum[(16 * dt + i) * 64];
       }
   }
-  if (key < pl.len) {
-    store_row<T, NDT, VEC>(DK + (int64_t)(pl.start + key) * a.k_st + (int64_t)hk * a.k_sh, D, g, dk, scale);
-    store_row<T, NDT, VEC>(DV + (int64_t)(pl.start + key) * a.v_st + (int64_t)hk * a.v_sh, D, g, dv, 1.f);
+  T* dk_at = DK + (int64_t)(pl.start + key) * a.k_st + (int64_t)hk * a.k_sh;
+  T* dv_at = DV + (int64_t)(pl.start + key) * a.v_st + (int64_t)hk * a.v_sh;
+  const bool bad_k = any_not_finite(dk, key < pl.len), bad_v = any_not_finite(dv, key < pl.len);
+  if (bad_k || bad_v) {
+    T* w = reinterpret_cast<T*>(wave & 2 ? Q1 : Q0) + (wave & 1) * 1024;
+    dkv_again<T, NKS, NDT, A, true>(Qb, Kr, Vr, Db, LSE2 + stat0, DELTA + stat0, dk_at, w, a.q_st, a.q_sh, a.o_st,
+                                    a.o_sh, a.total, G, D, rows, key0, key < pl.len, sl2, scale, lane);
+    dkv_again<T, NKS, NDT, A, false>(Qb, Kr, Vr, Db, LSE2 + stat0, DELTA + stat0, dv_at, w, a.q_st, a.q_sh, a.o_st,
+                                     a.o_sh, a.total, G, D, rows, key0, key < pl.len, sl2, 1.f, lane);
+  } else if (key < pl.len) {
+    store_row<T, NDT, A>(dk_at, D, g, dk, scale);
+    store_row<T, NDT, A>(dv_at, D, g, dv, 1.f);
   }
 }
 
 // ---------------------------------------------------------------- launches
 namespace {
 
-template <class T, int NKS, int NDT, bool VEC>
+template <class T, int NKS, int NDT, int A>
 hipError_t fwd_t(const void* q, const void* k, const void* v, void* o, float* lse, PackedArgs a, float scale,
                  hipStream_t stream) {
   a.slots = packed_slots(a, 128, a.G);
   TimingScope ts("packed_fwd", stream);
-  hipLaunchKernelGGL((packed_fwd_kernel<T, NKS, NDT, VEC>), dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream,
+  hipLaunchKernelGGL((packed_fwd_kernel<T, NKS, NDT, A>), dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream,
                      static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
                      static_cast<T*>(o), lse, a, (float)((double)scale * 1.4426950408889634));
   return hipGetLastError();
 }
 
-template <class T, int NKS, int NDT, bool VEC>
+template <class T, int NKS, int NDT, int A>
 hipError_t bwd_t(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
                  void* dq, void* dk, void* dv, float* ws, PackedArgs a, float scale, hipStream_t stream) {
   const float sl2 = (float)((double)scale * 1.4426950408889634);
@@ -781,7 +932,7 @@ hipError_t bwd_t(const void* q, const void* k, const void* v, const void* o, con
   {
     TimingScope ts("packed_bwd_dq", stream);
     a.slots = packed_slots(a, 128, a.G);
-    hipLaunchKernelGGL((packed_dq_kernel<T, NKS, NDT, VEC>), dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream,
+    hipLaunchKernelGGL((packed_dq_kernel<T, NKS, NDT, A>), dim3((unsigned)a.slots * a.HK), dim3(256), 0, stream,
                        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
                        static_cast<const T*>(o), static_cast<const T*>(d_o), lse, static_cast<T*>(dq), lse2, delta, a,
                        sl2, scale);
@@ -799,34 +950,37 @@ hipError_t bwd_t(const void* q, const void* k, const void* v, const void* o, con
   // of up to 64), or without one (they fill a CU alone)
   if constexpr (sizeof(T) * NDT <= 8) {
     if ((int64_t)a.total * a.HK < (sizeof(T) * NDT <= 4 ? 512 : 128) * 128) {
-      launch(packed_dkv_kernel<T, NKS, NDT, 2, VEC>, 64);
+      launch(packed_dkv_kernel<T, NKS, NDT, 2, A>, 64);
       return hipGetLastError();
     }
   }
-  launch(packed_dkv_kernel<T, NKS, NDT, 4, VEC>, 128);
+  launch(packed_dkv_kernel<T, NKS, NDT, 4, A>, 128);
   return hipGetLastError();
 }
 
-// NKS: steps of 16 over the head dim, NDT: 32-wide tiles of it
-#define WHA_BY_DIM(F, T, D, vec, ...)                       \
-  (D) <= 64 ? ((vec) ? F<T, 4, 2, true>(__VA_ARGS__) : F<T, 4, 2, false>(__VA_ARGS__)) \
-            : ((vec) ? F<T, 8, 4, true>(__VA_ARGS__) : F<T, 8, 4, false>(__VA_ARGS__))
+// F<T, steps of 16 over the head dim, 32-wide tiles of it, alignment of rows>
+#define WHA_BY_DIM(F, T, ...)                                                                     \
+  (a.D <= 64 ? (align == 16  ? F<T, 4, 2, 16>(__VA_ARGS__)                                        \
+                : align == 4 ? F<T, 4, 2, 4>(__VA_ARGS__)                                         \
+                             : F<T, 4, 2, sizeof(T) == 4 ? 4 : 2>(__VA_ARGS__))                   \
+             : (align == 16  ? F<T, 8, 4, 16>(__VA_ARGS__)                                        \
+                : align == 4 ? F<T, 8, 4, 4>(__VA_ARGS__)                                         \
+                             : F<T, 8, 4, sizeof(T) == 4 ? 4 : 2>(__VA_ARGS__)))
 
 }  // namespace
 
 hipError_t launch_packed_fwd(int dtype, const void* q, const void* k, const void* v, void* o, float* lse,
-                             const PackedArgs& a, bool vec, float scale, hipStream_t stream) {
-  if (dtype == kF32) return WHA_BY_DIM(fwd_t, float, a.D, vec, q, k, v, o, lse, a, scale, stream);
-  if (dtype == kBf16) return WHA_BY_DIM(fwd_t, __bf16, a.D, vec, q, k, v, o, lse, a, scale, stream);
-  return WHA_BY_DIM(fwd_t, _Float16, a.D, vec, q, k, v, o, lse, a, scale, stream);
+                             const PackedArgs& a, int align, float scale, hipStream_t stream) {
+  if (dtype == kF32) return WHA_BY_DIM(fwd_t, float, q, k, v, o, lse, a, scale, stream);
+  if (dtype == kBf16) return WHA_BY_DIM(fwd_t, __bf16, q, k, v, o, lse, a, scale, stream);
+  return WHA_BY_DIM(fwd_t, _Float16, q, k, v, o, lse, a, scale, stream);
 }
 
 hipError_t launch_packed_bwd(int dtype, const void* q, const void* k, const void* v, const void* o, const void* d_o,
-                             const float* lse, void* dq, void* dk, void* dv, float* ws, const PackedArgs& a, bool vec,
+                             const float* lse, void* dq, void* dk, void* dv, float* ws, const PackedArgs& a, int align,
                              float scale, hipStream_t stream) {
-  if (dtype == kF32)
-    return WHA_BY_DIM(bwd_t, float, a.D, vec, q, k, v, o, d_o, lse, dq, dk, dv, ws, a, scale, stream);
-  return WHA_BY_DIM(bwd_t, __bf16, a.D, vec, q, k, v, o, d_o, lse, dq, dk, dv, ws, a, scale, stream);
+  if (dtype == kF32) return WHA_BY_DIM(bwd_t, float, q, k, v, o, d_o, lse, dq, dk, dv, ws, a, scale, stream);
+  return WHA_BY_DIM(bwd_t, __bf16, q, k, v, o, d_o, lse, dq, dk, dv, ws, a, scale, stream);
 }
 
 }  // namespace wha

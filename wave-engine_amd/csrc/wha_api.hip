@@ -1467,12 +1467,28 @@ bool rows_aligned(size_t size, std::initializer_list<const wha_layout*> views,
   return true;
 }
 
-// 32-bit byte offsets within 64 positions of these views, all heads included
-bool tile_offsets_fit(size_t size, std::initializer_list<const wha_layout*> views) {
-  for (const wha_layout* L : views)
-    if ((L->stride_t + L->stride_h) > ((int64_t)1 << 31) ||
-        (64 * L->stride_t + L->H * L->stride_h + L->D) * (int64_t)size >= (int64_t)1 << 31)
+// 16 or 4: every row of these views starts at a multiple of so many bytes and is one
+// long; else 2 (a 16-bit element).
+int rows_align(size_t size, std::initializer_list<const wha_layout*> views, std::initializer_list<const void*> ptrs) {
+  for (const int bytes : {16, 4}) {
+    bool ok = true;
+    for (const wha_layout* L : views)
+      for (const int64_t n : {(int64_t)L->D, L->stride_t, L->H > 1 ? L->stride_h : 0})
+        ok = ok && n * (int64_t)size % bytes == 0;
+    for (const void* p : ptrs) ok = ok && reinterpret_cast<uintptr_t>(p) % bytes == 0;
+    if (ok) return bytes;
+  }
+  return 2;
+}
+// Whether 32-bit byte offsets reach 64 positions of these views, and `heads` heads
+// further on.
+bool tile_offsets_fit(size_t size, std::initializer_list<const wha_layout*> views, int heads) {
+  for (const wha_layout* L : views) {
+    const int64_t most = ((int64_t)1 << 31) / (int64_t)size;
+    if (L->stride_t >= most / 64 || (heads > 1 && L->stride_h >= most / heads) ||
+        64 * L->stride_t + (heads > 1 ? (heads - 1) * L->stride_h : 0) + L->D >= most)
       return false;
+  }
   return true;
 }
 
@@ -1498,6 +1514,8 @@ int check_packed(const char* fn, const int32_t* cu, int32_t n_seq, int32_t dtype
   if ((int64_t)q->T * q->H >= ((int64_t)1 << 31) - (1 << 16) ||
       wha::packed_slots64(q->T, n_seq, 128, G) * k->H >= ((int64_t)1 << 31))
     return fail(WHA_ERR_UNSUPPORTED, "%s: rows x heads, or sequences x heads, too large", fn);
+  if (!tile_offsets_fit(wha::elem_size(dtype), {k, v}, 1))
+    return fail(WHA_ERR_UNSUPPORTED, "%s: 64 rows of k or v span 2 GiB", fn);
   *a = wha::PackedArgs{cu, n_seq, q->T, k->H, G, q->D, 0, q->stride_t, q->stride_h, k->stride_t, k->stride_h,
                        v->stride_t, v->stride_h, o->stride_t, o->stride_h};
   return WHA_OK;
@@ -1553,10 +1571,9 @@ int wha_packed_fwd(const void* q, const void* k, const void* v, void* o, float* 
   const int rc = check_packed(fn, cu_seqlens, n_seq, dtype, q_layout, k_layout, v_layout, o_layout, scale, &a);
   if (rc) return rc;
   if (!q || !k || !v || !o) return fail(WHA_ERR_INVALID, "%s: q, k, v and o must be non-NULL", fn);
-  const bool vec = rows_aligned(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout}, {q, k, v, o}) &&
-                   tile_offsets_fit(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout});
+  const int align = rows_align(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout}, {q, k, v, o});
   const hipError_t e =
-      wha::launch_packed_fwd(dtype, q, k, v, o, lse, a, vec, scale, static_cast<hipStream_t>(stream));
+      wha::launch_packed_fwd(dtype, q, k, v, o, lse, a, align, scale, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "wha_packed_fwd launch");
   g_err[0] = 0;
   return WHA_OK;
@@ -1580,15 +1597,16 @@ int wha_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
                 "or WHA_F32", fn);
   if (!q || !k || !v || !o || !d_o || !lse || !dq || !dk || !dv)
     return fail(WHA_ERR_INVALID, "%s: every tensor pointer must be non-NULL", fn);
-  const bool vec = rows_aligned(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout},
-                                {q, k, v, o, d_o, dq, dk, dv}) &&
-                   tile_offsets_fit(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout});
+  if (!tile_offsets_fit(wha::elem_size(dtype), {q_layout, o_layout}, a.G))
+    return fail(WHA_ERR_UNSUPPORTED, "%s: 64 rows of the heads of a group span 2 GiB in q or o", fn);
+  const int align = rows_align(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout},
+                               {q, k, v, o, d_o, dq, dk, dv});
   hipStream_t s = static_cast<hipStream_t>(stream);
   void* ws = nullptr;
   if ((rc = resolve_workspace(workspace, workspace_bytes, wha_packed_bwd_workspace_size(q_layout), s, fn, &ws)))
     return rc;
   const hipError_t e = wha::launch_packed_bwd(dtype, q, k, v, o, d_o, lse, dq, dk, dv, static_cast<float*>(ws), a,
-                                              vec, scale, s);
+                                              align, scale, s);
   if (e != hipSuccess) return hip_fail(e, "wha_packed_bwd launch");
   g_err[0] = 0;
   return WHA_OK;

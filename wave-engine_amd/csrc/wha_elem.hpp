@@ -100,6 +100,78 @@ struct Elem<_Float16> {
   }
 };
 
+// The products of the packed operators.  16-bit types: as they are.  float: on the
+// bf16 matrix cores at fp32 precision, each number as three bf16 parts, x = h + m +
+// l, of whose nine products the six that reach fp32 precision are summed (Henry,
+// Tang and Heinecke, "Leveraging the bfloat16 artificial intelligence datatype for
+// higher-precision computations", 2019): 192 cycles for what takes the fp32 MFMA
+// 512.  The small products go to an accumulator of their own, added once at the
+// end: a small product added to a large sum would lose its low bits each time.  The
+// parts of an infinity hold NaN, so results that are not finite are formed again
+// in Elem's arithmetic.
+template <class T>
+struct Fast {
+  typedef typename Elem<T>::Frag Frag;
+  struct Sum {
+    floatx16 big;
+    __device__ __forceinline__ Sum() { zero(); }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) big[i] = 0.f;
+    }
+    __device__ __forceinline__ void add(const Frag& a, const Frag& b) { big = Elem<T>::mma32(a, b, big); }
+    __device__ __forceinline__ floatx16 value() const { return big; }
+  };
+  __device__ __forceinline__ static Frag pack(const float (&x)[8]) { return Elem<T>::pack(x); }
+};
+struct Frag3 {
+  bf16x8 h, m, l;
+};
+template <>
+struct Fast<float> {
+  typedef Frag3 Frag;
+  typedef Elem<__bf16> B;
+  struct Sum {
+    floatx16 big, small;
+    __device__ __forceinline__ Sum() {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) big[i] = small[i] = 0.f;
+    }
+    __device__ __forceinline__ void add(const Frag& a, const Frag& b) {
+      small = B::mma32(a.l, b.h, small);
+      small = B::mma32(a.h, b.l, small);
+      small = B::mma32(a.m, b.m, small);
+      small = B::mma32(a.m, b.h, small);
+      small = B::mma32(a.h, b.m, small);
+      big = B::mma32(a.h, b.h, big);
+    }
+    __device__ __forceinline__ floatx16 value() const {
+      floatx16 x;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = big[i] + small[i];
+      return x;
+    }
+  };
+  // a pair rounded to bf16 (first in the low half), leaving what remains of it
+  __device__ __forceinline__ static unsigned take(float& a, float& b) {
+    const unsigned h = B::pair(a, b);
+    a -= __uint_as_float(h << 16);
+    b -= __uint_as_float(h & 0xffff0000u);
+    return h;
+  }
+  __device__ __forceinline__ static Frag pack(const float (&x)[8]) {
+    uintx4 h, m, l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a = x[2 * i], b = x[2 * i + 1];
+      h[i] = take(a, b);
+      m[i] = take(a, b);
+      l[i] = B::pair(a, b);
+    }
+    return Frag{__builtin_bit_cast(bf16x8, h), __builtin_bit_cast(bf16x8, m), __builtin_bit_cast(bf16x8, l)};
+  }
+};
+
 // Keeps what is formed from x where it stands in program order (an empty
 // statement that x passes through).  The addresses that a tile's reads are made
 // from are formed again for every tile, from a pinned lane: held in registers
@@ -116,19 +188,6 @@ __device__ __forceinline__ floatx16 zeros16() {
 }
 // Row within a 32 x 32 result of element i of lane group g.
 __device__ __forceinline__ int row32(int i, int g) { return 8 * (i >> 2) + 4 * g + (i & 3); }
-
-// A bit set where an element of a register is an infinity or NaN: an exponent of
-// all ones, plus one, carries into the sign's place (and no further).
-template <class T>
-__device__ __forceinline__ unsigned not_finite_bits(unsigned x) {
-  constexpr unsigned e = std::is_same<T, float>::value      ? 0x7f800000u
-                         : std::is_same<T, _Float16>::value ? 0x7c007c00u
-                                                            : 0x7f807f80u;
-  constexpr unsigned one = std::is_same<T, float>::value      ? 0x00800000u
-                           : std::is_same<T, _Float16>::value ? 0x04000400u
-                                                              : 0x00800080u;
-  return ((x & e) + one) & (sizeof(T) == 4 ? 0x80000000u : 0x80008000u);
-}
 
 // A tile of rows of DP elements in LDS, read both as the rows operand of
 // contractions over d (8 consecutive d of one row per lane) and as the columns
@@ -226,6 +285,36 @@ struct LdsTile {
   // element d of row r
   __device__ __forceinline__ static float one(const char* t, int r, int d) {
     return (float)*reinterpret_cast<const T*>(t + at(r, d / Elem<T>::kQuad) + (d % Elem<T>::kQuad) * (int)sizeof(T));
+  }
+};
+
+// A tile of ROWS fp32 rows in its three bf16 parts, each a tile of its own.
+template <int DP, int ROWS>
+struct SplitTile {
+  typedef LdsTile<__bf16, DP> Part;
+  static constexpr int kPart = ROWS * Part::kRow, kRow = 3 * Part::kRow;
+  __device__ __forceinline__ static Frag3 rows32(const char* t, int r0, int ks, int lane) {
+    return Frag3{Part::rows32(t, r0, ks, lane), Part::rows32(t + kPart, r0, ks, lane),
+                 Part::rows32(t + 2 * kPart, r0, ks, lane)};
+  }
+  __device__ __forceinline__ static Frag3 cols32(const char* t, int ks, int dt, int lane) {
+    return Frag3{Part::cols32(t, ks, dt, lane), Part::cols32(t + kPart, ks, dt, lane),
+                 Part::cols32(t + 2 * kPart, ks, dt, lane)};
+  }
+  // elements 4 q .. 4 q + 3 of row r
+  __device__ __forceinline__ static void put4(char* t, int r, int q, floatx4 x) {
+    uintx2 h, m, l;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float a = x[2 * i], b = x[2 * i + 1];
+      h[i] = Fast<float>::take(a, b);
+      m[i] = Fast<float>::take(a, b);
+      l[i] = Elem<__bf16>::pair(a, b);
+    }
+    char* p = t + Part::at(r, q >> 1) + 8 * (q & 1);
+    *reinterpret_cast<uintx2*>(p) = h;
+    *reinterpret_cast<uintx2*>(p + kPart) = m;
+    *reinterpret_cast<uintx2*>(p + 2 * kPart) = l;
   }
 };
 

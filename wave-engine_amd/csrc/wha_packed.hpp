@@ -24,11 +24,13 @@ struct PackedArgs {
 inline int64_t packed_slots64(int64_t total, int n_seq, int BM, int G) { return total * G / BM + n_seq; }
 inline int packed_slots(const PackedArgs& a, int BM, int G) { return (int)packed_slots64(a.total, a.n_seq, BM, G); }
 
+// align: 16 or 4 where every row of every tensor is (and D elements are) a multiple
+// of so many bytes, else 2.
 hipError_t launch_packed_fwd(int dtype, const void* q, const void* k, const void* v, void* o, float* lse,
-                             const PackedArgs& a, bool vec, float scale, hipStream_t stream);
+                             const PackedArgs& a, int align, float scale, hipStream_t stream);
 // ws: 2 * total * n_head floats.
 hipError_t launch_packed_bwd(int dtype, const void* q, const void* k, const void* v, const void* o, const void* d_o,
-                             const float* lse, void* dq, void* dk, void* dv, float* ws, const PackedArgs& a, bool vec,
+                             const float* lse, void* dq, void* dk, void* dv, float* ws, const PackedArgs& a, int align,
                              float scale, hipStream_t stream);
 
 // Paged cache: [n_pages][HK][P][D] elements of `cache_dtype` in k and v, P = 1 <<
