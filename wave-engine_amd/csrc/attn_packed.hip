@@ -90,6 +90,9 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
   return p;
 }
 
+// Kernels whose registers are full: addresses are formed again for every tile.
+template <class T, int DP>
+constexpr bool kTight = DP > 64 || sizeof(T) == 4;
 // The LDS tiles that the products read.
 template <class T, int DP, int ROWS>
 using Tile = typename std::conditional<sizeof(T) == 4, SplitTile<DP, ROWS>, LdsTile<T, DP>>::type;
@@ -106,6 +109,7 @@ constexpr int kPast = (int)0x80000000;
 template <class T, int DP, int ROWS, int NT, int A>
 struct Stage {
   using L = Tile<T, DP, ROWS>;
+  static constexpr bool PIN = kTight<T, DP>;
   static constexpr int kRow = DP * (int)sizeof(T);  // bytes of a row in memory, padded
   static constexpr int UNIT = sizeof(T) == 2 && A == 4 ? 4 : 16, UPR = kRow / UNIT, PER = ROWS * UPR / NT;
   static_assert(ROWS * UPR % NT == 0, "whole rounds");
@@ -113,7 +117,7 @@ struct Stage {
 
   template <class Off>
   __device__ __forceinline__ void begin(__amdgpu_buffer_rsrc_t r, char* lds, int D, int tid, Off&& off) {
-    pin(tid);
+    if constexpr (PIN) pin(tid);
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int i = p * NT + tid, rr = i / UPR, u = i % UPR;
@@ -155,11 +159,32 @@ struct Stage {
       }
     }
   }
-  // rows row0 .. of one head, st elements apart, n of them in all
+  // Rows row0 .. of one head, st elements apart, n of them in all.  Where the rounds of
+  // the block's threads lie whole groups of 16 rows apart a lane has one offset, the
+  // same in every round and tile, and each round a descriptor of its own.
+  static constexpr int ROUND = NT / UPR;  // rows of a round
   __device__ __forceinline__ void begin_head(const T* base, int row0, int n, int64_t st, char* lds, int D, int tid) {
-    const int64_t left = ((int64_t)(min(n - row0, ROWS) - 1) * st + D) * (int64_t)sizeof(T);
-    begin(buffer_rsrc(base + (int64_t)row0 * st, (uint32_t)left), lds, D, tid,
-          [&](int rr) { return rr * (int)st * (int)sizeof(T); });
+    if constexpr (UNIT == 16 && A == 16 && (sizeof(T) == 4 || ROUND % 16 == 0)) {
+      const int rr = tid / UPR, u = tid % UPR;
+      int d = 4 * u;
+      if constexpr (sizeof(T) == 2) d = 8 * (u ^ L::swz(rr));
+      const int off = d < D ? (rr * (int)st + d) * (int)sizeof(T) : kPast;
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const int first = row0 + p * ROUND, rows = min(n - first, ROUND);
+        const uint32_t left = rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * st + D) * (int64_t)sizeof(T)) : 0u;
+        const __amdgpu_buffer_rsrc_t r = buffer_rsrc(base + (int64_t)first * st, left);
+        if constexpr (sizeof(T) == 4)
+          x[p] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+        else
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              r, (void __attribute__((address_space(3)))*)(lds + (p * NT + (tid & ~63)) * 16), 16, off, 0, 0, 0);
+      }
+    } else {
+      const int64_t left = ((int64_t)(min(n - row0, ROWS) - 1) * st + D) * (int64_t)sizeof(T);
+      begin(buffer_rsrc(base + (int64_t)row0 * st, (uint32_t)left), lds, D, tid,
+            [&](int rr) { return rr * (int)st * (int)sizeof(T); });
+    }
   }
 };
 
@@ -523,7 +548,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NDT <= 2 ? 3 : waves_per_sim
   auto tile = [&](int kt, const char* Kt, const char* Vt) {
     const int k0 = kt * KT;
     int ln = lane;
-    pin(ln);
+    if constexpr (kTight<T, DP>) pin(ln);
     floatx16 s[NSUB];
     typename F::Sum sum;
     one_ahead<NSUB * NKS>([&](int i) { return L::rows32(Kt, 32 * (i / NKS), i % NKS, ln); },
@@ -548,7 +573,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NDT <= 2 ? 3 : waves_per_sim
     // stay far from fp32's and P from its type's limits, and most tiles need no
     // rescaling
     if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
-      const float mn = vmax2(m, mx), alpha = mn == m ? 1.f : fast_exp2(m - mn);
+      const float mn = vmax2(m, mx);
+      float alpha = mn == m ? 1.f : fast_exp2(m - mn);
+      pin(alpha);  // (else the products are formed before the branch, every time)
       m = mn;
       l *= alpha;
 #pragma unroll
@@ -656,7 +683,7 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
     constexpr bool SUMS = decltype(sums)::value;  // the sweep that sums Delta
     const int k0 = kt * KT;
     int ln = lane;
-    pin(ln);
+    if constexpr (kTight<T, DP>) pin(ln);
     floatx16 ds[NSUB];
     const bool cut = k0 + KT - 1 > t_first;
 #pragma unroll
@@ -772,7 +799,7 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
     auto at = [&](int rr, int64_t st, int64_t sh) {
       int t, gq;
       place(rr, t, gq);
-      return (t * (int)st + gq * (int)sh) * (int)sizeof(T);
+      return ((int)__umul24(t, (int)st) + gq * (int)sh) * (int)sizeof(T);  // (64 st is below 2^31 / size)
     };
     qs_.begin(buffer_rsrc(Qb + (int64_t)t0 * a.q_st, 0x7fffffffu), Qd, D, tid,
               [&](int rr) { return at(rr, a.q_st, a.q_sh); });
@@ -813,7 +840,7 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
   auto tile = [&](int x, const char* Qt, const char* Dt, const float* St) {
     const int r0 = x * 32;
     int ln = lane;
-    pin(ln);
+    if constexpr (kTight<T, DP>) pin(ln);
     floatx16 p[1], ds[1];
     {
       typename F::Sum s;

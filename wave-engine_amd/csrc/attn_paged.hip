@@ -494,7 +494,9 @@ __global__ __launch_bounds__(256, REACH == kOnePage && sizeof(Product<T, C>) == 
     mx = vmax3(vmax3(mx, s[1][1], s[1][2]), s[1][3], s[1][3]);
     mx = pair_max32(pair_max16(mx)) * sl2;
     if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {  // (as in the packed forward)
-      const float mn = vmax2(m, mx), alpha = mn == m ? 1.f : fast_exp2(m - mn);
+      const float mn = vmax2(m, mx);
+      float alpha = mn == m ? 1.f : fast_exp2(m - mn);
+      pin(alpha);  // (else the products are formed before the branch, every time)
       m = mn;
       l *= alpha;
 #pragma unroll
