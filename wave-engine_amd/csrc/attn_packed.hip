@@ -37,6 +37,7 @@ namespace {
 // many balance by themselves.  Either way the grid needs only the total.
 struct Place {
   int tile, start, len;  // tile < 0: none left
+  int most;              // tiles of the longest sequence (of this one, where there are more than 64)
 };
 __device__ __forceinline__ int seq_start(const int* cu, int i, int total) { return min(max(cu[i], 0), total); }
 template <bool KEYS>
@@ -60,7 +61,7 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
       int count = 0;  // tiles of level x and higher
       for (int i = 0; i < n_seq; ++i) count += max(0, __builtin_amdgcn_readlane(n, i) - x);
       const int c = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(count > order)) - 1;
-      if (c < 0) return Place{-1, 0, 0};  // fewer tiles than this in all
+      if (c < 0) return Place{-1, 0, 0, 0};  // fewer tiles than this in all
       level += c * step;
       if (c < 63) above = __builtin_amdgcn_readlane(count, c + 1);
     }
@@ -70,6 +71,7 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
     p.start = __builtin_amdgcn_readlane(start, seq);
     p.len = __builtin_amdgcn_readlane(len, seq);
     p.tile = KEYS ? __builtin_amdgcn_readlane(n, seq) - 1 - level : level;
+    p.most = most;
     return p;
   }
   const int slot = KEYS ? order : slots - 1 - order;
@@ -87,6 +89,7 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
   p.len = __builtin_amdgcn_readfirstlane(max(0, seq_start(cu, lo + 1, total) - p.start));
   p.tile = slot - (int)((int64_t)p.start * G / BM) - lo;
   if ((int64_t)p.tile * BM >= (int64_t)p.len * G) p.tile = -1;
+  p.most = (int)(((int64_t)p.len * G + BM - 1) / BM);
   return p;
 }
 
@@ -558,10 +561,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NDT <= 2 ? 3 : waves_per_sim
                             if (i % NKS == NKS - 1) s[i / NKS] = sum.value();
                           });
     if (k0 + KT - 1 > t_first) {  // wave-uniform: the mask cuts through the tile
+      int mine = t;
+      pin(mine);  // (else the masks are formed before the branch, every time)
 #pragma unroll
       for (int x = 0; x < NSUB; ++x)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[x][i] = k0 + 32 * x + row32(i, g) > t ? -INFINITY : s[x][i];
+        for (int i = 0; i < 16; ++i) s[x][i] = k0 + 32 * x + row32(i, g) > mine ? -INFINITY : s[x][i];
     }
     float mx = s[0][0];
 #pragma unroll
@@ -702,8 +707,10 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
         ds[x][i] = SUMS ? p * dv[i] : p * (dv[i] - delta);
       }
       if (cut) {
+        int mine = t;
+        pin(mine);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ds[x][i] = k0 + 32 * x + row32(i, g) > t ? 0.f : ds[x][i];
+        for (int i = 0; i < 16; ++i) ds[x][i] = k0 + 32 * x + row32(i, g) > mine ? 0.f : ds[x][i];
       }
     }
     if constexpr (SUMS) {
@@ -719,7 +726,7 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
     auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
       if constexpr (sizeof(T) == 2) wait_vmem();
       __syncthreads();
-      if (kt + 1 < n_kt) begin(kt + 1, Kn, Vn);
+        if (kt + 1 < n_kt) begin(kt + 1, Kn, Vn);
       if (kt < n_w) tile(sums, kt, Kt, Vt);
       if (kt + 1 < n_kt) end(Kn, Vn);
     };
@@ -756,7 +763,7 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
 // and are added up at the end (KG = 2: where blocks of 128 keys are too few for the
 // CUs).
 template <class T, int NKS, int NDT, int KG, int A>
-__global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dkv_kernel(
+__global__ __launch_bounds__(256, sizeof(T) == 4 || (NDT > 2 && KG == 2) ? 1 : 2) void packed_dkv_kernel(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ DO,
     const float* __restrict__ LSE2, const float* __restrict__ DELTA, T* __restrict__ DK, T* __restrict__ DV,
     PackedArgs a, float sl2, float scale) {
@@ -779,7 +786,7 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
   const Place pl = find_place<true>(a.cu, a.n_seq, a.total, 1, BN, a.slots, (int)(blockIdx.x / a.HK), lane);
   if (pl.tile < 0) return;
   const int rows = pl.len * G, key0 = pl.tile * BN + kg * 32;
-  const int key = key0 + (lane & 31), kc = min(key, pl.len - 1);
+  const int key = key0 + (lane & 31);
   const int first = key * G;  // the first row that comes at or after the key
   const T* Qb = Q + (int64_t)pl.start * a.q_st + (int64_t)hk * G * a.q_sh;
   const T* Db = DO + (int64_t)pl.start * a.o_st + (int64_t)hk * G * a.o_sh;
@@ -801,10 +808,10 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
       place(rr, t, gq);
       return ((int)__umul24(t, (int)st) + gq * (int)sh) * (int)sizeof(T);  // (64 st is below 2^31 / size)
     };
-    qs_.begin(buffer_rsrc(Qb + (int64_t)t0 * a.q_st, 0x7fffffffu), Qd, D, tid,
-              [&](int rr) { return at(rr, a.q_st, a.q_sh); });
-    ds_.begin(buffer_rsrc(Db + (int64_t)t0 * a.o_st, 0x7fffffffu), Dd, D, tid,
-              [&](int rr) { return at(rr, a.o_st, a.o_sh); });
+    const __amdgpu_buffer_rsrc_t rq = buffer_rsrc(Qb + (int64_t)t0 * a.q_st, 0x7fffffffu);
+    const __amdgpu_buffer_rsrc_t rd = buffer_rsrc(Db + (int64_t)t0 * a.o_st, 0x7fffffffu);
+    qs_.begin(rq, Qd, D, tid, [&](int rr) { return at(rr, a.q_st, a.q_sh); });
+    ds_.begin(rd, Dd, D, tid, [&](int rr) { return at(rr, a.o_st, a.o_sh); });
     if (wave < RG) {  // 64 of the 2 QT statistics to a wave
       int t, gq;
       place((wave * 64 + lane) % QT, t, gq);
@@ -824,12 +831,15 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
   const char* Vw = VS + kg * 32 * LV::kRow;
 
   typename F::Frag kf[NKS], vf[V_LDS ? 1 : NKS];
-  const T* Kr = K + (int64_t)(pl.start + kc) * a.k_st + (int64_t)hk * a.k_sh;
-  const T* Vr = Vb + (int64_t)kc * a.v_st;
+  {
+    const int kc = min(key, pl.len - 1);
+    const T* Kr = K + (int64_t)(pl.start + kc) * a.k_st + (int64_t)hk * a.k_sh;
+    const T* Vr = Vb + (int64_t)kc * a.v_st;
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) {
-    kf[ks] = fast_of<T>(row8<T, A>(Kr, 16 * ks + 8 * g, D));
-    if constexpr (!V_LDS) vf[ks] = fast_of<T>(row8<T, A>(Vr, 16 * ks + 8 * g, D));
+    for (int ks = 0; ks < NKS; ++ks) {
+      kf[ks] = fast_of<T>(row8<T, A>(Kr, 16 * ks + 8 * g, D));
+      if constexpr (!V_LDS) vf[ks] = fast_of<T>(row8<T, A>(Vr, 16 * ks + 8 * g, D));
+    }
   }
   end(Q0, D0);
   floatx16 dk[NDT], dv[NDT];
@@ -870,12 +880,17 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
         p[0][i] = fast_exp2(fmaf(p[0][i], sl2, -lse2[e]));
         ds[0][i] = p[0][i] * (ds[0][i] - delta[e]);
       }
+      // (no more of the statistics in registers: one spill in this loop is a wait for
+      // all loads in flight, the next tile's)
+      WHA_FENCE();
     }
     if (is_cut(x)) {
+      int from = first;
+      pin(from);  // (else the masks are formed before the branch, every time)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int row = r0 + row32(i, g);
-        const bool in = row >= first && row < rows;
+        const bool in = row >= from && row < rows;
         p[0][i] = in ? p[0][i] : 0.f;
         ds[0][i] = in ? ds[0][i] : 0.f;
       }
@@ -888,6 +903,7 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
   auto step = [&](int rt, char* Qt, char* Dt, float* St, char* Qn, char* Dn, float* Sn) {
     wait_vmem();
     __syncthreads();
+    prio_by_remaining(n_rt - rt, pl.most * BN / QT * G);
     if (rt + 1 < n_rt) begin(rt + 1, Qn, Dn, Sn);
     const int x = rt * RG + rg;
     if (x >= sub0 && x * 32 < rows) tile(x, Qt + own, Dt + own, St + rg * 32);
@@ -922,18 +938,25 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dk
         dv[dt][i] += v_sum[(16 * dt + i) * 64];
       }
   }
-  T* dk_at = DK + (int64_t)(pl.start + key) * a.k_st + (int64_t)hk * a.k_sh;
-  T* dv_at = DV + (int64_t)(pl.start + key) * a.v_st + (int64_t)hk * a.v_sh;
-  const bool bad_k = any_not_finite(dk, key < pl.len), bad_v = any_not_finite(dv, key < pl.len);
+  // (the lane's addresses once more: kept over the loop they would be spilled, or K)
+  int ln = lane;
+  pin(ln);
+  const int my_key = key0 + (ln & 31), row = pl.start + min(my_key, pl.len - 1);
+  const bool on = my_key < pl.len;
+  T* dk_at = DK + (int64_t)row * a.k_st + (int64_t)hk * a.k_sh;
+  T* dv_at = DV + (int64_t)row * a.v_st + (int64_t)hk * a.v_sh;
+  const bool bad_k = any_not_finite(dk, on), bad_v = any_not_finite(dv, on);
   if (bad_k || bad_v) {
+    const T* Kr = K + (int64_t)row * a.k_st + (int64_t)hk * a.k_sh;
+    const T* Vr = V + (int64_t)row * a.v_st + (int64_t)hk * a.v_sh;
     T* w = reinterpret_cast<T*>(wave & 2 ? Q1 : Q0) + (wave & 1) * 1024;
     dkv_again<T, NKS, NDT, A, true>(Qb, Kr, Vr, Db, LSE2 + stat0, DELTA + stat0, dk_at, w, a.q_st, a.q_sh, a.o_st,
-                                    a.o_sh, a.total, G, D, rows, key0, key < pl.len, sl2, scale, lane);
+                                    a.o_sh, a.total, G, D, rows, key0, on, sl2, scale, ln);
     dkv_again<T, NKS, NDT, A, false>(Qb, Kr, Vr, Db, LSE2 + stat0, DELTA + stat0, dv_at, w, a.q_st, a.q_sh, a.o_st,
-                                     a.o_sh, a.total, G, D, rows, key0, key < pl.len, sl2, 1.f, lane);
-  } else if (key < pl.len) {
-    store_row<T, NDT, A>(dk_at, D, g, dk, scale);
-    store_row<T, NDT, A>(dv_at, D, g, dv, 1.f);
+                                     a.o_sh, a.total, G, D, rows, key0, on, sl2, 1.f, ln);
+  } else if (on) {
+    store_row<T, NDT, A>(dk_at, D, ln >> 5, dk, scale);
+    store_row<T, NDT, A>(dv_at, D, ln >> 5, dv, 1.f);
   }
 }
 
@@ -976,7 +999,7 @@ hipError_t bwd_t(const void* q, const void* k, const void* v, const void* o, con
   // blocks of 64 keys where 128 would leave CUs without a second block (16-bit rows
   // of up to 64), or without one (they fill a CU alone)
   if constexpr (sizeof(T) * NDT <= 8) {
-    if ((int64_t)a.total * a.HK < (sizeof(T) * NDT <= 4 ? 512 : 128) * 128) {
+    if ((int64_t)a.total * a.HK < (sizeof(T) * NDT <= 8 && !(sizeof(T) == 2 && NDT > 2) ? 512 : 128) * 128) {
       launch(packed_dkv_kernel<T, NKS, NDT, 2, A>, 64);
       return hipGetLastError();
     }
