@@ -19,6 +19,7 @@
 // += V^T P^T as it stands; with keys kept (dK, dV) as S = Q K^T, for the same
 // reason.
 #include <hip/hip_runtime.h>
+#include <utility>
 
 #include "wha_elem.hpp"
 #include "wha_packed.hpp"
@@ -31,13 +32,14 @@ namespace {
 // A tile's level is the number of tiles that it sweeps less one: those before it in
 // its sequence, or with KEYS (tiles of keys, swept by the rows after them) those
 // after it.  Up to 64 sequences: the highest level first, whatever the sequence, so
-// that the longest sweeps start first and the short ones fill in behind them.  More
+// that the longest sweeps start first and the short ones fill in behind them (16
+// ragged sequences of up to 1024, 12 heads of 64 in 4 groups: 28 us, one sequence
+// after the other 36).  More
 // sequences: sequence i has the slots from floor(rows before it / BM) + i on, which
 // is at least as many as it has tiles; that needs no sum over the sequences, and so
 // many balance by themselves.  Either way the grid needs only the total.
 struct Place {
   int tile, start, len;  // tile < 0: none left
-  int most;              // tiles of the longest sequence (of this one, where there are more than 64)
 };
 __device__ __forceinline__ int seq_start(const int* cu, int i, int total) { return min(max(cu[i], 0), total); }
 template <bool KEYS>
@@ -61,7 +63,7 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
       int count = 0;  // tiles of level x and higher
       for (int i = 0; i < n_seq; ++i) count += max(0, __builtin_amdgcn_readlane(n, i) - x);
       const int c = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(count > order)) - 1;
-      if (c < 0) return Place{-1, 0, 0, 0};  // fewer tiles than this in all
+      if (c < 0) return Place{-1, 0, 0};  // fewer tiles than this in all
       level += c * step;
       if (c < 63) above = __builtin_amdgcn_readlane(count, c + 1);
     }
@@ -71,7 +73,6 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
     p.start = __builtin_amdgcn_readlane(start, seq);
     p.len = __builtin_amdgcn_readlane(len, seq);
     p.tile = KEYS ? __builtin_amdgcn_readlane(n, seq) - 1 - level : level;
-    p.most = most;
     return p;
   }
   const int slot = KEYS ? order : slots - 1 - order;
@@ -89,7 +90,6 @@ __device__ __forceinline__ Place find_place(const int* cu, int n_seq, int total,
   p.len = __builtin_amdgcn_readfirstlane(max(0, seq_start(cu, lo + 1, total) - p.start));
   p.tile = slot - (int)((int64_t)p.start * G / BM) - lo;
   if ((int64_t)p.tile * BM >= (int64_t)p.len * G) p.tile = -1;
-  p.most = (int)(((int64_t)p.len * G + BM - 1) / BM);
   return p;
 }
 
@@ -258,53 +258,65 @@ __device__ __forceinline__ void store_row(T* dst, int D, int g, const floatx16 (
     }
 }
 
-// N steps whose operands come from LDS: the reads of step i + 1 go out before the
-// MFMAs of step i, no more of them, so that they cost few registers.
-template <int N, class Load, class Use>
-__device__ __forceinline__ void one_ahead(Load&& load, Use&& use) {
-  auto f = load(0);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    auto next = f;
-    if (i + 1 < N) next = load(i + 1);
-    use(i, f);
-    WHA_FENCE();
-    f = next;
-  }
+// N steps whose operands come from LDS: the reads of step i + AHEAD go out before
+// the MFMAs of step i, no more of them, so that they cost few registers.  Two steps
+// where the MFMAs of one take less than an LDS read (a fence behind the reads, or the
+// scheduler puts them after the MFMAs and the next ones wait out their latency:
+// forward of 64 x 4096 x 128 423 us without, 374 with), one for the six products of
+// fp32 (no fence: 48 us against 58 with, for want of registers).
+template <class T>
+inline constexpr int kAhead = sizeof(T) == 4 ? 1 : 2;
+template <class F, int... I>
+__device__ __forceinline__ void each(std::integer_sequence<int, I...>, F&& f) {
+  (f(std::integral_constant<int, I>()), ...);
 }
-template <class F, int N>
-struct Frags {
-  F f[N];
+template <class T, int FROM, int TO, int AHEAD = kAhead<T>, class Load, class Use>
+__device__ __forceinline__ void ahead(Load&& load, Use&& use) {
+  constexpr int N = TO - FROM;
+  decltype(load(std::integral_constant<int, FROM>())) f[AHEAD + 1];
+  each(std::make_integer_sequence<int, AHEAD>(), [&](auto i) { f[i] = load(std::integral_constant<int, FROM + i>()); });
+  each(std::make_integer_sequence<int, N>(), [&](auto i) {
+    if constexpr (i + AHEAD < N)
+      f[(i + AHEAD) % (AHEAD + 1)] = load(std::integral_constant<int, FROM + i + AHEAD>());
+    if constexpr (sizeof(T) == 2) WHA_FENCE();
+    use(std::integral_constant<int, FROM + i>(), f[i % (AHEAD + 1)]);
+    WHA_FENCE();
+  });
+}
+
+// What a step reads: one or two fragments and its elements' statistics.
+template <class F, int E>
+struct Step {
+  F a, b;
+  float stat[E];
 };
 
-// acc[d][column] += sum over the tile's 32 NSUB rows of p[row][column] x[row][d].
-template <class T, class L, int NDT, int NSUB>
-__device__ __forceinline__ void add_cols(const char* t, const floatx16 (&p)[NSUB], floatx16 (&acc)[NDT], int lane) {
-  constexpr int N = 2 * NSUB;
-  typename Fast<T>::Frag f[N];
+// p's two fragments of 16 rows, the weights of an MFMA with the tile's columns
+template <class T>
+__device__ __forceinline__ void pack_rows(const floatx16& p, typename Fast<T>::Frag (&f)[2]) {
 #pragma unroll
-  for (int s = 0; s < N; ++s) {
-    float x[8];
+  for (int b = 0; b < 2; ++b) {
+    float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = p[s / 2][8 * (s & 1) + j];
-    f[s] = Fast<T>::pack(x);
+    for (int j = 0; j < 8; ++j) y[j] = p[8 * b + j];
+    f[b] = Fast<T>::pack(y);
   }
-  auto cols = [&](int i) { return L::cols32(t, i % N, i / N, lane); };
+}
+// Step j of acc[d][column] += sum over 16 N rows of p[row][column] x[row][d]: N steps
+// to each 32 columns of x, x the rows 16 (j % N) .. of them, f their p.
+template <class T, int N = 2, int NDT>
+__device__ __forceinline__ void add_cols(int j, const typename Fast<T>::Frag& x, const typename Fast<T>::Frag (&f)[2],
+                                         floatx16 (&acc)[NDT], typename Fast<T>::Sum& sum) {
   if constexpr (sizeof(T) == 4) {
-    typename Fast<T>::Sum sum;
-    one_ahead<N * NDT>(cols, [&](int i, const typename Fast<T>::Frag& x) {
-      if (i % N == 0) sum = typename Fast<T>::Sum();
-      sum.add(x, f[i % N]);
-      if (i % N == N - 1) {
-        const floatx16 y = sum.value();
+    if (j % N == 0) sum = typename Fast<T>::Sum();
+    sum.add(x, f[j % 2]);
+    if (j % N == N - 1) {
+      const floatx16 y = sum.value();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i / N][e] += y[e];
-      }
-    });
+      for (int e = 0; e < 16; ++e) acc[j / N][e] += y[e];
+    }
   } else {
-    one_ahead<N * NDT>(cols, [&](int i, const typename Fast<T>::Frag& x) {
-      acc[i / N] = Elem<T>::mma32(x, f[i % N], acc[i / N]);
-    });
+    acc[j / N] = Elem<T>::mma32(x, f[j % 2], acc[j / N]);
   }
 }
 
@@ -497,19 +509,22 @@ __device__ __forceinline__ void dkv_again(const T* Qb, const T* Kr, const T* Vr,
   if (on) store_row<T, NDT, A>(to, D, g, acc, scale);
 }
 
-// Waves to a SIMD that the kernels' loops leave room for in its registers (fp32: three
-// parts of two operands and a result of 128 fill them).
-constexpr int waves_per_simd(int size, int ndt) { return size == 4 && ndt > 2 ? 1 : 2; }
-
 }  // namespace
 
 // ---------------------------------------------------------------- forward
+// A tile of K and one of V at a time, two of each in LDS; a wave keeps 32 queries' Q,
+// maximum, sum and O^T in registers.  16 bits, 32 query heads of 128 in 8 groups, 4
+// sequences of 4096: 373 us, 0.86 PFLOP/s of the products that the mask leaves; the
+// matrix cores are busy 45% of it, the VALU (exponentials, maxima) as long, and the
+// two overlap only where a wave's own instructions alternate.  Waves to a SIMD: as
+// many as the loop's registers leave room for.
 template <class T, int NKS, int NDT, int A>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && NDT <= 2 ? 3 : waves_per_simd(sizeof(T), NDT)) void packed_fwd_kernel(
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (NDT <= 2 ? 3 : 2) : (NDT <= 2 ? 2 : 1)) void packed_fwd_kernel(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, T* __restrict__ O,
     float* __restrict__ LSE, PackedArgs a, float sl2) {
   constexpr int DP = 32 * NDT, NT = 256, BM = 128, KT = sizeof(T) == 4 ? 32 : 64, NSUB = KT / 32;
   using L = Tile<T, DP, KT>;
+  using E = Elem<T>;
   using F = Fast<T>;
   constexpr int BYTES = KT * L::kRow;
   __shared__ __align__(16) char K0[BYTES], K1[BYTES], V0[BYTES], V1[BYTES];
@@ -554,49 +569,72 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NDT <= 2 ? 3 : waves_per_sim
     if constexpr (kTight<T, DP>) pin(ln);
     floatx16 s[NSUB];
     typename F::Sum sum;
-    one_ahead<NSUB * NKS>([&](int i) { return L::rows32(Kt, 32 * (i / NKS), i % NKS, ln); },
-                          [&](int i, const typename F::Frag& f) {
-                            if (i % NKS == 0) sum = typename F::Sum();
-                            sum.add(f, qf[i % NKS]);
-                            if (i % NKS == NKS - 1) s[i / NKS] = sum.value();
-                          });
-    if (k0 + KT - 1 > t_first) {  // wave-uniform: the mask cuts through the tile
-      int mine = t;
-      pin(mine);  // (else the masks are formed before the branch, every time)
+    typename F::Frag f[2];
+    const bool cut = k0 + KT - 1 > t_first;  // the mask cuts through the tile
+    float mx = -INFINITY, sub = 0.f;
+    auto weigh = [&](int x, int i) {
+      s[x][i] = fast_exp2(fmaf(s[x][i], sl2, -sub));
+      l += s[x][i];
+    };
+    // the scores of the tile's rows, 32 by 32, beside them the maximum of the last 32;
+    // then O += P V, beside it the weights of the next 32
+    constexpr int S = NSUB * NKS, C = 2 * NDT, E = 16 / NKS;
+    static_assert(NKS == C, "as many steps to a product as to the other");
+    ahead<T, 0, S + NSUB * C>(
+        [&](auto i) {
+          return i < S ? L::rows32(Kt, 32 * (i / NKS), i % NKS, ln)
+                       : L::cols32(Vt, 2 * ((i - S) / C) + i % 2, (i - S) % C / 2, ln);
+        },
+        [&](auto i, const typename F::Frag& y) {
+          if (i < S) {
+            const int x = i / NKS, ks = i % NKS;
+            if (ks == 0) sum = typename F::Sum();
+            sum.add(y, qf[ks]);
+            if (x > 0)
 #pragma unroll
-      for (int x = 0; x < NSUB; ++x)
+              for (int e = 0; e < E; ++e) mx = vmax2(mx, s[x - 1][E * ks + e]);
+            if (ks == NKS - 1) {
+              s[x] = sum.value();
+              if (cut) {  // wave-uniform
+                int mine = t - k0;
+                pin(mine);  // (else the masks are formed before the branch, every time)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[x][i] = k0 + 32 * x + row32(i, g) > mine ? -INFINITY : s[x][i];
-    }
-    float mx = s[0][0];
+                for (int e = 0; e < 16; ++e) s[x][e] = 32 * x + row32(e, g) > mine ? -INFINITY : s[x][e];
+              }
+            }
+            if (i == S - 1) {
 #pragma unroll
-    for (int x = 0; x < NSUB; ++x)
+              for (int e = 0; e < 16; ++e) mx = vmax2(mx, s[x][e]);
+              mx = pair_max32(mx) * sl2;
+              // O and l keep the maximum they have until one passes it by 2^8: the sums
+              // stay far from fp32's and P from its type's limits, and most tiles need no
+              // rescaling
+              if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
+                const float mn = vmax2(m, mx);
+                float alpha = mn == m ? 1.f : fast_exp2(m - mn);
+                pin(alpha);  // (else the products are formed before the branch, every time)
+                m = mn;
+                l *= alpha;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = vmax2(mx, s[x][i]);
-    mx = pair_max32(mx) * sl2;
-    // O and l keep the maximum they have until one passes it by 2^8: the sums
-    // stay far from fp32's and P from its type's limits, and most tiles need no
-    // rescaling
-    if (__builtin_amdgcn_ballot_w64(mx > m + 8.f) != 0) {
-      const float mn = vmax2(m, mx);
-      float alpha = mn == m ? 1.f : fast_exp2(m - mn);
-      pin(alpha);  // (else the products are formed before the branch, every time)
-      m = mn;
-      l *= alpha;
+                for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
+                  for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+              }
+              sub = m == -INFINITY ? 0.f : m;  // only scores of -inf so far: weights of 0
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
-    }
-    const float sub = m == -INFINITY ? 0.f : m;  // only scores of -inf so far: weights of 0
+              for (int e = 0; e < 16; ++e) weigh(0, e);
+              pack_rows<T>(s[0], f);
+            }
+          } else {
+            const int x = (i - S) / C, j = (i - S) % C;
+            add_cols<T>(j, y, f, o, sum);
+            if (x + 1 < NSUB) {
 #pragma unroll
-    for (int x = 0; x < NSUB; ++x)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[x][i] = fast_exp2(fmaf(s[x][i], sl2, -sub));
-        l += s[x][i];
-      }
-    add_cols<T, L>(Vt, s, o, ln);
+              for (int e = 0; e < E; ++e) weigh(x + 1, E * j + e);
+              if (j == C - 1) pack_rows<T>(s[x + 1], f);
+            }
+          }
+        });
   };
   auto step = [&](int kt, char* Kt, char* Vt, char* Kn, char* Vn) {
     if constexpr (sizeof(T) == 2) wait_vmem();
@@ -629,9 +667,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NDT <= 2 ? 3 : waves_per_sim
 // Delta = do . o takes o as the forward rounded it; in 16 bits the error is as large
 // as that of the rounded score gradients where a row has few keys.  Blocks whose
 // rows all lie below kShort sum Delta over p dp in a sweep of its own instead.
+//
+// 16 bits, 32 query heads of 128 in 8 groups, 4 sequences of 4096: 480 us, 1.0
+// PFLOP/s of its three products; bound as the forward is.  fp32 takes one wave to a
+// SIMD: 45 us for 16 sequences of up to 512, 8 heads of 48, with two (and spills) 48.
 constexpr int kShort = 256;
 template <class T, int NKS, int NDT, int A>
-__global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq_kernel(
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void packed_dq_kernel(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ O,
     const T* __restrict__ DO, const float* __restrict__ LSE, T* __restrict__ DQ, float* __restrict__ LSE2,
     float* __restrict__ DELTA, PackedArgs a, float sl2, float scale) {
@@ -689,37 +731,55 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
     const int k0 = kt * KT;
     int ln = lane;
     if constexpr (kTight<T, DP>) pin(ln);
-    floatx16 ds[NSUB];
     const bool cut = k0 + KT - 1 > t_first;
-#pragma unroll
-    for (int x = 0; x < NSUB; ++x) {
-      typename F::Sum s, dp;
-      typedef Frags<typename F::Frag, 2> F2;
-      one_ahead<NKS>([&](int ks) { return F2{{L::rows32(Kt, 32 * x, ks, ln), L::rows32(Vt, 32 * x, ks, ln)}}; },
-                     [&](int ks, const F2& f) {
-                       s.add(f.f[0], qf[ks]);
-                       dp.add(f.f[1], dof[ks]);
-                     });
-      const floatx16 sv = s.value(), dv = dp.value();
+    // the scores and dO V^T of 32 keys after 32, two chains of MFMAs side by side, and
+    // dS = p (dO V^T - Delta); then dQ += dS K
+    typename F::Frag f[NSUB][2];
+    floatx16 all[NSUB];
+    typedef Step<typename F::Frag, 1> Reads;
+    each(std::make_integer_sequence<int, NSUB>(), [&](auto x) {
+      typename F::Sum sum, dsum;
+      ahead<T, 0, NKS>(
+          [&](auto ks) {
+            Reads y;
+            y.a = L::rows32(Kt, 32 * x, ks, ln);
+            y.b = L::rows32(Vt, 32 * x, ks, ln);
+            return y;
+          },
+          [&](auto ks, const Reads& y) {
+            sum.add(y.a, qf[ks]);
+            dsum.add(y.b, dof[ks]);
+          });
+      const floatx16 s = sum.value(), dp = dsum.value();
+      floatx16 ds;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float p = fast_exp2(fmaf(sv[i], sl2, -lse2));
-        ds[x][i] = SUMS ? p * dv[i] : p * (dv[i] - delta);
+        const float p = fast_exp2(fmaf(s[i], sl2, -lse2));
+        ds[i] = SUMS ? p * dp[i] : p * (dp[i] - delta);
       }
       if (cut) {
         int mine = t;
-        pin(mine);
+        pin(mine);  // (else the masks are formed before the branch, every time)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ds[x][i] = k0 + 32 * x + row32(i, g) > mine ? 0.f : ds[x][i];
+        for (int i = 0; i < 16; ++i) ds[i] = k0 + 32 * x + row32(i, g) > mine ? 0.f : ds[i];
       }
-    }
-    if constexpr (SUMS) {
+      if constexpr (SUMS) {
 #pragma unroll
-      for (int x = 0; x < NSUB; ++x)
+        for (int i = 0; i < 16; ++i) sum_delta += ds[i];
+      } else {
+        all[x] = ds;
+      }
+    });
+    if constexpr (!SUMS)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum_delta += ds[x][i];
-    } else {
-      add_cols<T, L>(Kt, ds, dq, ln);
+      for (int x = 0; x < NSUB; ++x) pack_rows<T>(all[x], f[x]);
+    if constexpr (!SUMS) {
+      constexpr int N = 2 * NSUB;
+      typename F::Sum sum;
+      ahead<T, 0, N * NDT>([&](auto i) { return L::cols32(Kt, i % N, i / N, ln); },
+                           [&](auto i, const typename F::Frag& y) {
+                             add_cols<T, N>(i, y, f[i % N / 2], dq, sum);
+                           });
     }
   };
   auto sweep = [&](auto sums) {
@@ -762,8 +822,15 @@ __global__ __launch_bounds__(256, waves_per_simd(sizeof(T), NDT)) void packed_dq
 // after them: KG waves of 32 keys each, times 4 / KG that take every other 32 rows
 // and are added up at the end (KG = 2: where blocks of 128 keys are too few for the
 // CUs).
+//
+// 16 bits, 32 query heads of 128 in 8 groups, 4 sequences of 4096: 1000 us, 0.64
+// PFLOP/s of its four products: dK, dV and K fill the registers (V is read from LDS
+// again for every tile), which leaves none to read ahead from one product to the next
+// or to form p and dS beside the MFMAs (1470 us: a spill among the loads in flight
+// waits for all of them).  64 columns leave them: 50 us for 12 sequences of up to
+// 1024, 12 heads of 64 in 4 groups, one product after the other 56.
 template <class T, int NKS, int NDT, int KG, int A>
-__global__ __launch_bounds__(256, sizeof(T) == 4 || (NDT > 2 && KG == 2) ? 1 : 2) void packed_dkv_kernel(
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void packed_dkv_kernel(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ DO,
     const float* __restrict__ LSE2, const float* __restrict__ DELTA, T* __restrict__ DK, T* __restrict__ DV,
     PackedArgs a, float sl2, float scale) {
@@ -851,59 +918,105 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (NDT > 2 && KG == 2) ? 1 : 2
     const int r0 = x * 32;
     int ln = lane;
     if constexpr (kTight<T, DP>) pin(ln);
-    floatx16 p[1], ds[1];
-    {
-      typename F::Sum s;
-      one_ahead<NKS>([&](int ks) { return L::rows32(Qt, 0, ks, ln); },
-                     [&](int ks, const typename F::Frag& f) { s.add(f, kf[ks]); });
-      p[0] = s.value();
-    }
-    {
-      typename F::Sum s;
-      if constexpr (V_LDS) {
-        typedef Frags<typename F::Frag, 2> F2;
-        one_ahead<NKS>([&](int ks) { return F2{{L::rows32(Dt, 0, ks, ln), LV::rows32(Vw, 0, ks, ln)}}; },
-                       [&](int ks, const F2& f) { s.add(f.f[0], f.f[1]); });
-      } else {
-        one_ahead<NKS>([&](int ks) { return L::rows32(Dt, 0, ks, ln); },
-                       [&](int ks, const typename F::Frag& f) { s.add(f, vf[ks]); });
-      }
-      ds[0] = s.value();
-    }
+    // the scores; V dO^T, beside it the weights p; dV += p dO, beside it
+    // dS = p (V dO^T - Delta), in dp's place; dK += dS Q
+    floatx16 p, dp;
+    typename F::Sum sum;
+    typename F::Frag f[2];
+    constexpr int C = 2 * NDT, E = 16 / NKS;
+    static_assert(NKS == C, "as many steps to a product as to the others");
+    constexpr bool BESIDE = NDT <= 2;  // where there are registers for it
+    typedef Step<typename F::Frag, E> Reads;
+    auto load = [&](auto i) {
+          Reads y;
+          const int k = i % NKS, el = E * k;
+          const float* st = St + 8 * (el / 4) + 4 * g + el % 4;
+          if (i < NKS) {
+            y.a = L::rows32(Qt, 0, k, ln);
+          } else if (i < 2 * NKS) {
+            y.a = L::rows32(Dt, 0, k, ln);
+            if constexpr (V_LDS) y.b = LV::rows32(Vw, 0, k, ln);
+            if constexpr (BESIDE)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const floatx4 lse2 = *reinterpret_cast<const floatx4*>(St + 8 * u + 4 * g);
-      const floatx4 delta = *reinterpret_cast<const floatx4*>(St + QT + 8 * u + 4 * g);
+              for (int e = 0; e < E; ++e) y.stat[e] = st[e];
+          } else if (i < 2 * NKS + C) {
+            y.a = L::cols32(Dt, k % 2, k / 2, ln);
+            if constexpr (BESIDE)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * u + e;
-        p[0][i] = fast_exp2(fmaf(p[0][i], sl2, -lse2[e]));
-        ds[0][i] = p[0][i] * (ds[0][i] - delta[e]);
-      }
-      // (no more of the statistics in registers: one spill in this loop is a wait for
-      // all loads in flight, the next tile's)
-      WHA_FENCE();
-    }
-    if (is_cut(x)) {
-      int from = first;
-      pin(from);  // (else the masks are formed before the branch, every time)
+              for (int e = 0; e < E; ++e) y.stat[e] = st[QT + e];
+          } else {
+            y.a = L::cols32(Qt, k % 2, k / 2, ln);
+          }
+          return y;
+        };
+    auto use = [&](auto i, const Reads& y) {
+          const int k = i % NKS;
+          if (i < 2 * NKS && k == 0) sum = typename F::Sum();
+          if (i < NKS) {
+            sum.add(y.a, kf[k]);
+            if (k == NKS - 1) p = sum.value();
+          } else if (i < 2 * NKS) {
+            if constexpr (V_LDS)
+              sum.add(y.a, y.b);
+            else
+              sum.add(y.a, vf[k]);
+            if constexpr (BESIDE)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int row = r0 + row32(i, g);
-        const bool in = row >= from && row < rows;
-        p[0][i] = in ? p[0][i] : 0.f;
-        ds[0][i] = in ? ds[0][i] : 0.f;
-      }
+              for (int e = 0; e < E; ++e) p[E * k + e] = fast_exp2(fmaf(p[E * k + e], sl2, -y.stat[e]));
+            if (k == NKS - 1) {
+              dp = sum.value();
+              if constexpr (!BESIDE) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  const floatx4 lse2 = *reinterpret_cast<const floatx4*>(St + 8 * u + 4 * g);
+                  const floatx4 delta = *reinterpret_cast<const floatx4*>(St + QT + 8 * u + 4 * g);
+#pragma unroll
+                  for (int e = 4 * u; e < 4 * u + 4; ++e) {
+                    p[e] = fast_exp2(fmaf(p[e], sl2, -lse2[e % 4]));
+                    dp[e] = p[e] * (dp[e] - delta[e % 4]);
+                  }
+                  // (no more of the statistics in registers: one spill in this loop is a wait
+                  // for all loads in flight, the next tile's)
+                  WHA_FENCE();
+                }
+              }
+              if (is_cut(x)) {
+                int from = first;
+                pin(from);  // (else the masks are formed before the branch, every time)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const int row = r0 + row32(e, g);
+                  const bool in = row >= from && row < rows;
+                  p[e] = in ? p[e] : 0.f;
+                  if constexpr (!BESIDE) dp[e] = in ? dp[e] : 0.f;
+                }
+              }
+              pack_rows<T>(p, f);
+            }
+          } else if (i < 2 * NKS + C) {
+            add_cols<T>(k, y.a, f, dv, sum);
+            if constexpr (BESIDE)
+#pragma unroll
+              for (int e = 0; e < E; ++e) dp[E * k + e] = p[E * k + e] * (dp[E * k + e] - y.stat[e]);
+            if (k == C - 1) pack_rows<T>(dp, f);
+          } else {
+            add_cols<T>(k, y.a, f, dk, sum);
+          }
+        };
+    if constexpr (BESIDE) {
+      ahead<T, 0, 2 * NKS + 2 * C>(load, use);
+    } else {  // (and no reads on the way from one product to the next)
+      ahead<T, 0, NKS, 1>(load, use);
+      ahead<T, NKS, 2 * NKS, 1>(load, use);
+      ahead<T, 2 * NKS, 2 * NKS + C, 1>(load, use);
+      ahead<T, 2 * NKS + C, 2 * NKS + 2 * C, 1>(load, use);
     }
-    add_cols<T, L>(Dt, p, dv, ln);
-    add_cols<T, L>(Qt, ds, dk, ln);
   };
   // rows 32 rg .. of a tile (fp32: of each of its parts)
   const int own = rg * 32 * (V_LDS ? L::kRow : LV::kRow);
   auto step = [&](int rt, char* Qt, char* Dt, float* St, char* Qn, char* Dn, float* Sn) {
     wait_vmem();
     __syncthreads();
-    prio_by_remaining(n_rt - rt, pl.most * BN / QT * G);
     if (rt + 1 < n_rt) begin(rt + 1, Qn, Dn, Sn);
     const int x = rt * RG + rg;
     if (x >= sub0 && x * 32 < rows) tile(x, Qt + own, Dt + own, St + rg * 32);
@@ -949,7 +1062,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (NDT > 2 && KG == 2) ? 1 : 2
   if (bad_k || bad_v) {
     const T* Kr = K + (int64_t)row * a.k_st + (int64_t)hk * a.k_sh;
     const T* Vr = V + (int64_t)row * a.v_st + (int64_t)hk * a.v_sh;
-    T* w = reinterpret_cast<T*>(wave & 2 ? Q1 : Q0) + (wave & 1) * 1024;
+    // (two row groups: a wave's own buffer, the other wave may still read its sums)
+    T* w = RG == 2 ? reinterpret_cast<T*>(kg ? Q1 : Q0) : reinterpret_cast<T*>(wave & 2 ? Q1 : Q0) + (wave & 1) * 1024;
     dkv_again<T, NKS, NDT, A, true>(Qb, Kr, Vr, Db, LSE2 + stat0, DELTA + stat0, dk_at, w, a.q_st, a.q_sh, a.o_st,
                                     a.o_sh, a.total, G, D, rows, key0, on, sl2, scale, ln);
     dkv_again<T, NKS, NDT, A, false>(Qb, Kr, Vr, Db, LSE2 + stat0, DELTA + stat0, dv_at, w, a.q_st, a.q_sh, a.o_st,
@@ -996,10 +1110,12 @@ hipError_t bwd_t(const void* q, const void* k, const void* v, const void* o, con
                        static_cast<const T*>(k), static_cast<const T*>(v), static_cast<const T*>(d_o), lse2, delta,
                        static_cast<T*>(dk), static_cast<T*>(dv), a, sl2, scale);
   };
-  // blocks of 64 keys where 128 would leave CUs without a second block (16-bit rows
-  // of up to 64), or without one (they fill a CU alone)
-  if constexpr (sizeof(T) * NDT <= 8) {
-    if ((int64_t)a.total * a.HK < (sizeof(T) * NDT <= 8 && !(sizeof(T) == 2 && NDT > 2) ? 512 : 128) * 128) {
+  // Blocks of 64 keys where those of 128 come to fewer than two to a CU: 12 sequences
+  // of up to 1024, 12 heads of 64 in 4 groups 63 us against 111, fp32 of 16 sequences
+  // of up to 512, 8 heads of 48 60 against 64.  Heads of more than 64 take 128 always:
+  // 4 sequences of 4096, 8 heads of 128 1090 us against 1556.
+  if constexpr (NDT <= 2) {
+    if ((int64_t)a.total * a.HK < 512 * 128) {
       launch(packed_dkv_kernel<T, NKS, NDT, 2, A>, 64);
       return hipGetLastError();
     }

@@ -282,10 +282,6 @@ struct LdsTile {
       *reinterpret_cast<typename Elem<T>::Frag*>(t + at(r, c)) = x;
     }
   }
-  // element d of row r
-  __device__ __forceinline__ static float one(const char* t, int r, int d) {
-    return (float)*reinterpret_cast<const T*>(t + at(r, d / Elem<T>::kQuad) + (d % Elem<T>::kQuad) * (int)sizeof(T));
-  }
 };
 
 // A tile of ROWS fp32 rows in its three bf16 parts, each a tile of its own.
