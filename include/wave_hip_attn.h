@@ -450,7 +450,8 @@ int wha_wave_kv_decode(const float* x, const wha_wave_weights* w, const wha_wave
  * heads, k_layout->H = v_layout->H key-value heads, which must divide them (at
  * most 128 query heads to one); query head h uses key-value head h / (H / Hkv).
  * The views may be columns of one fused projection's rows.  lse [H][T], natural
- * log, may be NULL.  Row count x query heads must be below 2^31 - 2^16.
+ * log, may be NULL.  Row count x query heads must be below 2^31 - 2^16, and 128
+ * rows of k or v must span less than 2 GiB.
  * An infinity or NaN in a row reaches that row's and later rows' outputs of its
  * own sequence, never an earlier one's.  cu_seqlens entries outside [0, T] are
  * taken as 0 or T; with entries that decrease the outputs are unspecified, but
@@ -469,7 +470,8 @@ size_t wha_packed_bwd_workspace_size(const wha_layout* q_layout);
  * summed over the query heads of a group) in the layouts of q, k and v, d_o in
  * that of o.  The gradients must not overlap each other or the inputs.
  * WHA_F32 and WHA_BF16; WHA_F16 is WHA_ERR_UNSUPPORTED: score gradients of a few
- * thousand keys lie below its smallest number.  Deterministic (no atomics).
+ * thousand keys lie below its smallest number.  64 rows of q or o, with the heads
+ * of a group, must span less than 2 GiB.  Deterministic (no atomics).
  * workspace as for wha_attn_bwd. */
 int wha_packed_bwd(const void* q, const void* k, const void* v, const void* o,
                    const void* d_o, const float* lse, void* dq, void* dk,

@@ -126,6 +126,57 @@ def test_not_finite_rows_reach_no_earlier_row(pkg, dtype, value, D):
             near("dk", dk[at + 1:140], (ref["dk"][0][at + 1:140], ref["dk"][1][at + 1:140]))
 
 
+@pytest.mark.parametrize("dtype,D", [(F32, 48), (BF16, 64), (BF16, 40), (BF16, 42)])
+def test_enough_keys_for_the_larger_blocks(pkg, dtype, D):
+    """8231 rows of 8 key-value heads; then with a NaN in one sequence, which the others do not see."""
+    lens = [1100, 1, 700, 1300, 900, 1200, 800, 1250, 980]
+    q, k, v, do, cu = make(lens, 8, 8, D, dtype, 14)
+    ref = packed(q, k, v, cu.tolist(), pkg.default_scale(D), do)
+    rest = torch.ones(sum(lens), dtype=torch.bool, device=DEV)
+    for spoil in (False, True):
+        if spoil:
+            v[2000, 5, 7] = float("nan")
+            rest[1801:3101] = False
+        o, lse = pkg.packed_fwd(q, k, v, cu)
+        for name, x in (("o", o),) + tuple(zip(("dq", "dk", "dv"), pkg.packed_bwd(q, k, v, o, do, lse, cu))):
+            near(name, x[rest], (ref[name][0][rest], ref[name][1][rest]))
+        near("lse", lse, ref["lse"])  # (no score holds it)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_large_values(pkg, dtype):
+    """Values of 2^100 with gradients of 2^-100: the bounds are relative, and no part of a split falls
+    below 2^-126 where it counts."""
+    q, k, v, do, cu = make([90, 40], 4, 2, 64, dtype, 15)
+    v, do = v * 2.0 ** 100, do * 2.0 ** -100
+    o, lse = pkg.packed_fwd(q, k, v, cu)
+    ref = packed(q, k, v, cu.tolist(), pkg.default_scale(64), do)
+    near("o", o, ref["o"])
+    for name, x in zip(("dq", "dk", "dv"), pkg.packed_bwd(q, k, v, o, do, lse, cu)):
+        up = 2.0 ** 100 if name == "dv" else 1.0
+        near(name, x.double() * up, (ref[name][0] * up, ref[name][1] * up))
+
+
+def test_two_streams_at_once(pkg):
+    """Calls that alternate between two streams, each with inputs of its own and no workspace passed."""
+    sets = [make(lens, 6, 2, 64, BF16, 50 + i) for i, lens in enumerate(([900, 700], [500, 40, 1000]))]
+
+    def both(q, k, v, do, cu):
+        o, lse = pkg.packed_fwd(q, k, v, cu)
+        return (o, lse) + pkg.packed_bwd(q, k, v, o, do, lse, cu)
+
+    want = [both(*x) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(both(*sets[i % 2]))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(x, want[i % 2])), i
+
+
 def test_offsets_past_32_bits(pkg):
     """Rows 2^17 elements apart: the last sequence lies past 2^32 bytes and 2^31 elements."""
     N, W, D = 17000, 1 << 17, 64

@@ -64,6 +64,22 @@ def test_packed_refusals(pkg, bwd):
         refused(INVALID, b"aligned", ws=ctypes.c_void_p((1 << 20) + 4))
 
 
+@no_device
+def test_rows_too_far_apart_are_refused(pkg):
+    """A tile is loaded with 31-bit byte offsets from one base: 128 rows of k and v, in the backward
+    64 rows of q and o with the heads of a group."""
+    for size, dtype in ((2, 1), (4, 0)):
+        far = (1 << 31) // (128 * size)
+        for name in "kv":
+            for bwd in (False, True):
+                assert packed(pkg, bwd, dtype=dtype, **{name: view(pkg, H=2, stride_t=far)}) == UNSUPPORTED
+                assert b"2 GiB" in pkg.lib().wha_last_error()
+        for name in "qo":
+            for lay in (view(pkg, stride_t=2 * far), view(pkg, stride_h=64 * far, stride_t=64)):
+                assert packed(pkg, True, dtype=dtype, **{name: lay}) == UNSUPPORTED
+                assert b"2 GiB" in pkg.lib().wha_last_error()
+
+
 def test_workspace_sizes(pkg):
     L = pkg.lib()
     assert L.wha_packed_bwd_workspace_size(ctypes.byref(view(pkg, N=1000, H=3))) >= 1000 * 3 * 8

@@ -586,6 +586,8 @@ def packed_bwd(q, k, v, o, do, lse, cu_seqlens, scale=None, workspace=None, dq=N
     bfloat16."""
     Lq, Lk, Lv, n_seq = _packed_views(q, k, v, cu_seqlens)
     Lo = _heads_layout(o, "o", q)
+    if do is None:
+        raise TypeError("do: expected a tensor")
     grads = []
     for t, g, name in ((q, dq, "dq"), (k, dk, "dk"), (v, dv, "dv"), (o, do, "do")):
         if g is None:

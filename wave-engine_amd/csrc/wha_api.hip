@@ -1480,13 +1480,13 @@ int rows_align(size_t size, std::initializer_list<const wha_layout*> views, std:
   }
   return 2;
 }
-// Whether 32-bit byte offsets reach 64 positions of these views, and `heads` heads
-// further on.
-bool tile_offsets_fit(size_t size, std::initializer_list<const wha_layout*> views, int heads) {
+// Whether 31-bit byte offsets reach `rows` positions of these views, the tile that a
+// kernel loads from one base, and `heads` heads further on.
+bool tile_offsets_fit(size_t size, std::initializer_list<const wha_layout*> views, int rows, int heads) {
   for (const wha_layout* L : views) {
     const int64_t most = ((int64_t)1 << 31) / (int64_t)size;
-    if (L->stride_t >= most / 64 || (heads > 1 && L->stride_h >= most / heads) ||
-        64 * L->stride_t + (heads > 1 ? (heads - 1) * L->stride_h : 0) + L->D >= most)
+    if (L->stride_t >= most / rows || (heads > 1 && L->stride_h >= most / heads) ||
+        rows * L->stride_t + (heads > 1 ? (heads - 1) * L->stride_h : 0) + L->D >= most)
       return false;
   }
   return true;
@@ -1514,8 +1514,8 @@ int check_packed(const char* fn, const int32_t* cu, int32_t n_seq, int32_t dtype
   if ((int64_t)q->T * q->H >= ((int64_t)1 << 31) - (1 << 16) ||
       wha::packed_slots64(q->T, n_seq, 128, G) * k->H >= ((int64_t)1 << 31))
     return fail(WHA_ERR_UNSUPPORTED, "%s: rows x heads, or sequences x heads, too large", fn);
-  if (!tile_offsets_fit(wha::elem_size(dtype), {k, v}, 1))
-    return fail(WHA_ERR_UNSUPPORTED, "%s: 64 rows of k or v span 2 GiB", fn);
+  if (!tile_offsets_fit(wha::elem_size(dtype), {k, v}, 128, 1))
+    return fail(WHA_ERR_UNSUPPORTED, "%s: 128 rows of k or v span 2 GiB", fn);
   *a = wha::PackedArgs{cu, n_seq, q->T, k->H, G, q->D, 0, q->stride_t, q->stride_h, k->stride_t, k->stride_h,
                        v->stride_t, v->stride_h, o->stride_t, o->stride_h};
   return WHA_OK;
@@ -1597,7 +1597,7 @@ int wha_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
                 "or WHA_F32", fn);
   if (!q || !k || !v || !o || !d_o || !lse || !dq || !dk || !dv)
     return fail(WHA_ERR_INVALID, "%s: every tensor pointer must be non-NULL", fn);
-  if (!tile_offsets_fit(wha::elem_size(dtype), {q_layout, o_layout}, a.G))
+  if (!tile_offsets_fit(wha::elem_size(dtype), {q_layout, o_layout}, 64, a.G))
     return fail(WHA_ERR_UNSUPPORTED, "%s: 64 rows of the heads of a group span 2 GiB in q or o", fn);
   const int align = rows_align(wha::elem_size(dtype), {q_layout, k_layout, v_layout, o_layout},
                                {q, k, v, o, d_o, dq, dk, dv});
