@@ -34,7 +34,7 @@ namespace {
 // after it.  Up to 64 sequences: the highest level first, whatever the sequence, so
 // that the longest sweeps start first and the short ones fill in behind them (16
 // ragged sequences of up to 1024, 12 heads of 64 in 4 groups: 28 us, one sequence
-// after the other 36).  More
+// after the other 35; dQ of 12 of them 33 and 41).  More
 // sequences: sequence i has the slots from floor(rows before it / BM) + i on, which
 // is at least as many as it has tiles; that needs no sum over the sequences, and so
 // many balance by themselves.  Either way the grid needs only the total.
@@ -666,7 +666,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (NDT <= 2 ? 3 : 2) : (NDT <= 
 //
 // Delta = do . o takes o as the forward rounded it; in 16 bits the error is as large
 // as that of the rounded score gradients where a row has few keys.  Blocks whose
-// rows all lie below kShort sum Delta over p dp in a sweep of its own instead.
+// rows all lie below kShort sum Delta over p dp in a sweep of its own instead: dQ of
+// 12 ragged sequences of up to 1024 is off by 1.7e-3 of its norm that way, by 2.5e-3
+// with Delta from o everywhere; a sequence of 1024 is swept a sixteenth longer.
 //
 // 16 bits, 32 query heads of 128 in 8 groups, 4 sequences of 4096: 480 us, 1.0
 // PFLOP/s of its three products; bound as the forward is.  fp32 takes one wave to a
